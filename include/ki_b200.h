@@ -65,7 +65,8 @@ typedef enum { KI_VOTE_ALL = 0, KI_VOTE_ANY = 1, KI_VOTE_UNI = 2, KI_VOTE_BALLOT
 /* Element types and binary operators (warp-level and device-wide entry points). */
 typedef enum {
     KI_I8 = 0, KI_U8 = 1, KI_I16 = 2, KI_U16 = 3, KI_I32 = 4, KI_U32 = 5,
-    KI_I64 = 6, KI_U64 = 7, KI_F32 = 8, KI_F64 = 9
+    KI_I64 = 6, KI_U64 = 7, KI_F32 = 8, KI_F64 = 9,
+    KI_F16 = 10, KI_BF16 = 11  /* the operators of a layer only: ki_quantize_rows and below it */
 } ki_dtype;
 typedef enum {
     KI_OP_ADD = 0, KI_OP_MAX = 1, KI_OP_MIN = 2, KI_OP_OR = 3, KI_OP_AND = 4, KI_OP_XOR = 5, KI_OP_MUL = 6
@@ -87,7 +88,8 @@ int ki_ctx_destroy(ki_ctx* ctx);
  * had no context to hold it (a communicator whose set-up failed). */
 const char* ki_last_error_string(const ki_ctx* ctx);
 /* Synchronises `stream`, returns KI_ERR_TIMEOUT if any device-side wait of this context ran out
- * since the last check (and clears the latch), KI_ERR_CUDA on an asynchronous CUDA error. */
+ * since the last check, KI_ERR_ARG if a kernel met an offset or a slot number (read on the device) that
+ * was out of range (and clears both latches), KI_ERR_CUDA on an asynchronous CUDA error. */
 int ki_ctx_check(ki_ctx* ctx, void* stream);
 /* Limit of every device-side wait of this context (default 2 s). */
 int ki_ctx_set_wait_timeout_ns(ki_ctx* ctx, uint64_t ns);
@@ -316,6 +318,72 @@ int ki_compact_gt_f32_sharded(ki_comm* comm, const float* d_x, size_t n_local, f
  * M, N multiples of 128 and 256, K a multiple of 128, pointers 16-byte aligned (KI_ERR_ARG). */
 int ki_gemm_e4m3_f32(ki_ctx* ctx, const uint8_t* d_A, const uint8_t* d_B, float* d_C, int M, int N, int K,
                      float scale_a, float scale_b, void* stream);
+
+/* ---- operators of a state-space layer served in 8 bits ---------------------------------------
+ * No counterpart in the reference.  A layer runs ki_quantize_rows and ki_gemm_i8 for its projections,
+ * ki_causal_conv on what comes out of the first and ki_selective_scan on what the convolution gives;
+ * the _step forms continue the same states one token at a time.
+ * Elements are KI_F32, KI_F16 or KI_BF16 (one type per call); sums, states of the scan and scales are
+ * Float32, and every result is rounded once.  Matrices are row-major with a leading dimension in
+ * elements; inner dimensions are contiguous.  16-byte aligned rows move with 16-byte accesses, others
+ * element by element, with the same results.  An output that overlaps an input or another output
+ * (their whole ranges, first byte to last) returns KI_ERR_ARG.  No scratch: calls of one context may
+ * run on several streams at once and be captured into any number of graphs.
+ *
+ * Packed sequences: sequence i of seqs holds rows [d_offsets[i], d_offsets[i+1]) (Int32, seqs + 1
+ * values that do not decrease; NULL: one sequence of all rows); rows outside every sequence are left as
+ * they were.  State slots: sequence i uses slot d_slots[i] of `slots` (Int32; NULL: slot i); a negative
+ * number marks padding, whose rows and state are left as they were.  Several sequences of one call must
+ * not name the same slot (which of them remains is not defined).  d_initial (one byte each; NULL: all
+ * nonzero): 0 starts the sequence from zeros whatever its slot holds.  The slot holds the state after
+ * the sequence's last row when the call is complete (an empty sequence: the state it started from).
+ * Offsets and slots live on the device and are checked there: a slot number of `slots` or more is taken as
+ * padding, offsets are clamped to the rows, nothing outside the arrays is touched, and ki_ctx_check
+ * reports KI_ERR_ARG. */
+/* Rows to int8: scale[r] = max|x[r, :]| / 127 and q = rint(x / scale[r]) (ties to even), both quotients
+ * in IEEE Float32, q in [-127, 127].  scale 0 (a row of zeros, or cols = 0) gives q = 0; a row with a NaN
+ * or an infinity has scale NaN or infinity (and q = 0 where x / scale is NaN or 0). */
+int ki_quantize_rows(ki_ctx* ctx, int dtype, const void* d_x, size_t rows, size_t cols, size_t ld, int8_t* d_q,
+                     size_t ldq, float* d_scale, void* stream);
+/* C[m, n] = (sum_k A[m, k] W[n, k]) * scale_a[m] * scale_w[n] + bias[n] with exact Int32 sums, on the
+ * tensor cores.  A: M x K (tokens), W: N x K (channels), int8 row-major; any sizes, strides and
+ * alignments (rows that are not 16-byte aligned are slower); K <= 131071; d_bias: Float32[N] or NULL;
+ * C: M x N of out_dtype.  K = 0 gives the bias. */
+int ki_gemm_i8(ki_ctx* ctx, const int8_t* d_A, size_t lda, const int8_t* d_W, size_t ldw, const float* d_scale_a,
+               const float* d_scale_w, const float* d_bias, int out_dtype, void* d_C, size_t ldc, size_t M, size_t N,
+               size_t K, void* stream);
+/* Causal depthwise convolution: y[t, d] = act(bias[d] + sum_j w[d, j] x[t - (width-1) + j, d]), positions
+ * before the sequence from its state or zero; act is z * sigmoid(z) when silu is nonzero.  width 2 to 8;
+ * d_w: channels x width, contiguous; d_bias: channels values or NULL.  d_state: slots of (width-1) x
+ * channels inputs, state_ld elements apart, of the same type, oldest first; NULL: every sequence starts
+ * from zeros and no state is kept. */
+int ki_causal_conv(ki_ctx* ctx, int dtype, const void* d_x, size_t ldx, const void* d_w, const void* d_bias, void* d_state,
+                   size_t state_ld, size_t slots, const int32_t* d_slots, const uint8_t* d_initial,
+                   const int32_t* d_offsets, size_t seqs, void* d_y, size_t ldy, size_t tokens, size_t channels,
+                   int width, int silu, void* stream);
+/* One token per row: row r continues slot d_slots[r]. */
+int ki_causal_conv_step(ki_ctx* ctx, int dtype, const void* d_x, size_t ldx, const void* d_w, const void* d_bias,
+                        void* d_state, size_t state_ld, size_t slots, const int32_t* d_slots, void* d_y, size_t ldy,
+                        size_t rows, size_t channels, int width, int silu, void* stream);
+/* Selective scan: with s = delta[t, d] + delta_bias[d] (softplus'd when softplus is nonzero),
+ *   h_t[n] = exp(s A[d, n]) h_{t-1}[n] + s u[t, d] B[t, g, n],
+ *   y[t, d] = (sum_n C[t, g, n] h_t[n] + D[d] u[t, d]) * z sigmoid(z),   z = z[t, d],
+ * for `states` values n (1 to 256) of every channel d; channel d belongs to group d / (channels / groups).
+ * u, delta, z, y: tokens x channels; B, C: tokens x (groups * states); A: channels x states, D and
+ * delta_bias: channels, Float32.  d_D, d_z and d_delta_bias may be NULL (0, no gate, 0).  d_state: slots of
+ * channels x states Float32, state_ld elements apart, or NULL as above. */
+int ki_selective_scan(ki_ctx* ctx, int dtype, const void* d_u, size_t ldu, const void* d_delta, size_t ldd,
+                      const float* d_A, const void* d_B, size_t ldb, const void* d_C, size_t ldc, const float* d_D,
+                      const void* d_z, size_t ldz, const float* d_delta_bias, int softplus, float* d_state,
+                      size_t state_ld, size_t slots, const int32_t* d_slots, const uint8_t* d_initial,
+                      const int32_t* d_offsets, size_t seqs, void* d_y, size_t ldy, size_t tokens, size_t channels,
+                      size_t states, size_t groups, void* stream);
+/* One token per row: row r continues slot d_slots[r]. */
+int ki_selective_scan_step(ki_ctx* ctx, int dtype, const void* d_u, size_t ldu, const void* d_delta, size_t ldd,
+                           const float* d_A, const void* d_B, size_t ldb, const void* d_C, size_t ldc, const float* d_D,
+                           const void* d_z, size_t ldz, const float* d_delta_bias, int softplus, float* d_state,
+                           size_t state_ld, size_t slots, const int32_t* d_slots, void* d_y, size_t ldy, size_t rows,
+                           size_t channels, size_t states, size_t groups, void* stream);
 
 /* ---- warp-level intrinsics over whole warps of an array -------------------------------------
  * Element i of the array is lane i % 32 of warp i / 32; n must be a multiple of 32.           */

@@ -1,0 +1,125 @@
+// ki/layer.cuh -- what the operators of a model's layer share (quantize.cu, causal_conv.cu,
+// selective_scan.cu, gemm_i8.cu): Float32 / Float16 / BFloat16 elements, the activations, packed
+// sequences with their state slots, and checks of arguments.
+//
+// Elements are read in their type, every sum, state and scale is Float32 (the int8 product: Int32),
+// and a result is rounded once, to nearest even, when it is stored.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "ki/intrinsics.cuh"
+
+namespace ki {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// V consecutive elements moved with one access of sizeof(T) * V bytes (at most 16).
+template <class T, int V>
+struct alignas(sizeof(T) * V) Vec {
+    T e[V];
+};
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
+    return *reinterpret_cast<const Vec<T, V>*>(p);
+}
+template <class T, int V>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& v) {
+    *reinterpret_cast<Vec<T, V>*>(p) = v;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^x with one instruction (2 ulp); results below 2^-126 are zero.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// x * sigmoid(x); -inf gives NaN as the formula does.
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + exp2_fast(-kLog2e * x)); }
+// log(1 + e^x); above 20 it is x to Float32's precision.
+__device__ __forceinline__ float softplus(float x) { return x > 20.0f ? x : log1pf(expf(x)); }
+
+// ---- packed sequences ---------------------------------------------------------------------------
+// Sequence i holds tokens [offsets[i], offsets[i+1]) of the packed rows; without offsets there is one
+// sequence of all rows.  Offsets are read on the device, so they are clamped to the rows there are
+// and never trusted.
+struct Sequences {
+    const int32_t* offsets;
+    const int32_t* slots;    // state slot of each sequence; negative: the sequence is padding; null: slot i
+    const uint8_t* initial;  // nonzero: the sequence continues from its slot; null: every sequence does
+    int count;
+    int tokens;
+    int64_t nslots;
+    uint32_t* status;
+
+    __device__ __forceinline__ int begin(int i) const {
+        return offsets ? min(max(offsets[i], 0), tokens) : (i == 0 ? 0 : tokens);
+    }
+    // Slot of sequence i, or -1 where it has none (padding, or a number that no slot has, which is latched).
+    __device__ __forceinline__ int64_t slot(int i) const {
+        const int64_t s = slots ? (int64_t)slots[i] : (int64_t)i;
+        if (s >= nslots) {
+            atomicOr(status, (uint32_t)KI_DEV_BAD_INDEX);
+            return -1;
+        }
+        return s;
+    }
+    __device__ __forceinline__ bool continues(int i) const { return initial ? initial[i] != 0 : true; }
+    // Latches offsets that decrease or leave the rows (run by one block).
+    __device__ __forceinline__ void check(int tid, int threads) const {
+        if (!offsets) return;
+        bool bad = false;
+        for (int i = tid; i <= count; i += threads) {
+            const int o = offsets[i];
+            bad |= o < 0 || o > tokens || (i > 0 && offsets[i - 1] > o);
+        }
+        if (bad) atomicOr(status, (uint32_t)KI_DEV_BAD_INDEX);
+    }
+};
+
+// ---- host side ------------------------------------------------------------------------------------
+// Bytes [lo, hi) of a strided array: the first byte of its first row to the last of its last.
+struct Span {
+    uintptr_t lo = 0, hi = 0;
+};
+inline Span span(const void* p, size_t rows, size_t ld, size_t cols, size_t elem) {
+    Span s;
+    if (!p || rows == 0 || cols == 0) return s;
+    s.lo = (uintptr_t)p;
+    s.hi = s.lo + ((rows - 1) * ld + cols) * elem;
+    return s;
+}
+inline bool overlap(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+
+inline size_t float_size(int dtype) { return dtype == KI_F32 ? 4 : dtype == KI_F16 || dtype == KI_BF16 ? 2 : 0; }
+
+// Whether every row of an array starts on a multiple of `bytes`.
+inline bool rows_aligned(const void* p, size_t ld, size_t elem, size_t bytes) {
+    return aligned(p, bytes) && (ld * elem) % bytes == 0;
+}
+
+// Calls f with a value of the element type of dtype (KI_F32, KI_F16 or KI_BF16).
+template <class F>
+inline int with_float_type(int dtype, F f) {
+    switch (dtype) {
+        case KI_F32: return f(float());
+        case KI_F16: return f(__half());
+        default: return f(__nv_bfloat16());
+    }
+}
+
+}  // namespace ki

@@ -11,7 +11,9 @@ Names and argument meanings follow the reference (epilliat/KernelIntrinsics.jl v
 * ``access`` / ``fence`` validate scope/ordering like ``@access`` / ``@fence`` and raise
   ``KIArgumentError`` (a ``ValueError``) where the reference raises ``ArgumentError``;
 * device-wide operations built from them: ``vcopy`` (copyto!), ``warpfold_reduce`` (sum),
-  ``warpreduce_scan`` (cumsum), ``vote_compact`` (filter/findall), ``fp8_gemm``.
+  ``warpreduce_scan`` (cumsum), ``vote_compact`` (filter/findall), ``fp8_gemm``;
+* the operators of a state-space layer served in 8 bits (no counterpart in the reference): ``quantize_rows``,
+  ``int8_gemm``, ``causal_conv`` / ``causal_conv_step``, ``selective_scan`` / ``selective_scan_step``.
 
 Every operation runs a hand-written sm_100a kernel from libki_b200.so; tensors are torch CUDA tensors
 (torch provides device memory and streams only).  There is no CPU path.
@@ -31,7 +33,8 @@ __all__ = [
     "KITimeoutError", "Context", "context", "warpsize", "get_warpsize", "devices", "shfl", "warpreduce",
     "warpfold", "vote", "vload", "vstore", "vload_multi", "vstore_multi", "generate_partN", "access",
     "message_pass", "vcopy", "vcopy_host", "reduce", "reduce_rows", "scan", "compact", "warpfold_reduce", "reduce_sum_i64", "warpreduce_scan", "warpreduce_scan_host", "vote_compact",
-    "fp8_gemm", "fill_uniform", "fill_int_range", "fill_bytes", "fill_normal", "fill_e4m3_uniform",
+    "fp8_gemm", "quantize_rows", "int8_gemm", "causal_conv", "causal_conv_step", "selective_scan",
+    "selective_scan_step", "fill_uniform", "fill_int_range", "fill_bytes", "fill_normal", "fill_e4m3_uniform",
 ]
 
 
@@ -769,6 +772,274 @@ def fp8_gemm(A, B, C=None, scale_a: float = 1.0, scale_b: float = 1.0, stream=No
     context(d).call("ki_gemm_e4m3_f32", _ptr(A), _ptr(B), _ptr(C), M, N, K, ctypes.c_float(scale_a),
                     ctypes.c_float(scale_b), _stream_ptr(stream, d))
     return C
+
+
+# ---------------------------------------------------------------------------------------------
+# operators of a state-space layer served in 8 bits
+# ---------------------------------------------------------------------------------------------
+def _bad(what: str):
+    return KIArgumentError(_abi.KI_ERR_ARG, what)
+
+
+def _float_code(name: str, dtype) -> int:
+    code = _abi.FLOAT_DTYPE.get(str(dtype)[6:])
+    if code is None:
+        raise _bad(f"{name}: float32, float16 or bfloat16 elements, not {dtype}")
+    return code
+
+
+def _rows(name: str, what: str, t, shape: tuple, dtype, device) -> int:
+    """The row stride of a 2-D ``t`` of this shape, type and device whose rows are contiguous."""
+    if t.device != device:
+        raise _bad(f"{name}: {what} is on {t.device}, the first argument on {device}")
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise _bad(f"{name}: {what} must be {dtype} {list(shape)}, not {t.dtype} {list(t.shape)}")
+    ld, inner = t.stride()
+    if (shape[1] > 1 and inner != 1) or (shape[0] > 1 and ld < shape[1]):
+        raise _bad(f"{name}: {what} must have contiguous rows that do not overlap")
+    return ld if shape[0] > 1 else shape[1]
+
+
+def _flat(name: str, what: str, t, shape: tuple, dtype, device):
+    """A pointer to ``t``, contiguous and of this shape, type and device; None stays None."""
+    if t is None:
+        return None
+    if t.device != device or t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise _bad(f"{name}: {what} must be {dtype} {list(shape)}, contiguous and on {device}")
+    return t.data_ptr()
+
+
+def _new(shape, dtype, device, stream):
+    """An output that belongs to the stream that writes it."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _state(name: str, state, inner: tuple, dtype, device, slots, count: int):
+    """(pointer, elements between slots, slots, pointer to the slot numbers) of a cache of states."""
+    torch = _torch()
+    if state is None:
+        if slots is not None:
+            raise _bad(f"{name}: slots without a state")
+        return None, 0, 0, None
+    if state.device != device or state.dtype != dtype or state.dim() != 3 or tuple(state.shape[1:]) != inner:
+        raise _bad(f"{name}: state must be {dtype} [slots, {inner[0]}, {inner[1]}] on {device}")
+    n, held = state.shape[0], inner[0] * inner[1]
+    if held and n and not state[0].is_contiguous():
+        raise _bad(f"{name}: every slot of the state must be contiguous")
+    ld = state.stride(0) if n > 1 else held
+    if ld < held:
+        raise _bad(f"{name}: slots of the state overlap")
+    if slots is None and n < count:
+        raise _bad(f"{name}: {n} state slots for {count} sequences")
+    return state.data_ptr(), ld, n, _flat(name, "slots", slots, (count,), torch.int32, device)
+
+
+def _sequences(name: str, offsets, initial, state, device):
+    """(sequences, pointer to the offsets, pointer to the initial flags)."""
+    torch = _torch()
+    if offsets is None:
+        count = 1
+    else:
+        if offsets.dim() != 1 or offsets.numel() < 1:
+            raise _bad(f"{name}: offsets must hold one value more than there are sequences")
+        count = offsets.numel() - 1
+    at = _flat(name, "offsets", offsets, (count + 1,), torch.int32, device)
+    if initial is not None:
+        if state is None:
+            raise _bad(f"{name}: initial without a state")
+        if initial.dtype not in (torch.bool, torch.uint8):
+            raise _bad(f"{name}: initial must be bool or uint8")
+        initial = _flat(name, "initial", initial, (count,), initial.dtype, device)
+    return count, at, initial
+
+
+def _silu(name: str, activation) -> int:
+    if activation not in (None, "silu"):
+        raise _bad(f"{name}: activation must be 'silu' or None")
+    return int(activation == "silu")
+
+
+def _matrix(name: str, what: str, t) -> tuple:
+    if t.dim() != 2:
+        raise _bad(f"{name}: {what} must be 2-D")
+    return tuple(t.shape)
+
+
+def quantize_rows(x, out=None, scale=None, stream=None):
+    """int8 rows with one scale each: scale[r] = max|x[r]| / 127, out[r] = rint(x[r] / scale[r]) (ties to
+    even, both quotients in Float32), for a 2-D Float32, Float16 or BFloat16 ``x`` with contiguous rows.
+    A row of zeros gives zeros and scale 0; a NaN or an infinity stays in the row's scale.
+    Returns (out, scale): int8 of x's shape, Float32 per row."""
+    torch = _torch()
+    d = _dev(x)
+    rows, cols = _matrix("quantize_rows", "x", x)
+    code = _float_code("quantize_rows", x.dtype)
+    ld = _rows("quantize_rows", "x", x, (rows, cols), x.dtype, x.device)
+    out = _new((rows, cols), torch.int8, x.device, stream) if out is None else out
+    scale = _new((rows,), torch.float32, x.device, stream) if scale is None else scale
+    ldq = _rows("quantize_rows", "out", out, (rows, cols), torch.int8, x.device)
+    ps = _flat("quantize_rows", "scale", scale, (rows,), torch.float32, x.device)
+    context(d).call("ki_quantize_rows", code, x.data_ptr(), rows, cols, ld, out.data_ptr(), ldq, ps,
+                    _stream_ptr(stream, d))
+    return out, scale
+
+
+def int8_gemm(A, W, scale_a, scale_w, bias=None, out=None, dtype=None, stream=None):
+    """out[m, n] = (sum_k A[m, k] W[n, k]) * scale_a[m] * scale_w[n] + bias[n] with exact Int32 sums on the
+    tensor cores: int8 tokens ``A`` (M x K) and weights ``W`` (N x K) with contiguous rows, Float32 scales per
+    token and per channel, Float32 ``bias`` or None.  ``out`` has ``dtype`` (bfloat16 unless given)."""
+    torch = _torch()
+    name = "int8_gemm"
+    d = _dev(A)
+    (M, K), (N, KW) = _matrix(name, "A", A), _matrix(name, "W", W)
+    if K != KW:
+        raise _bad(f"{name}: inner dimensions differ")
+    if dtype is None:
+        dtype = torch.bfloat16 if out is None else out.dtype
+    code = _float_code(name, dtype)
+    lda = _rows(name, "A", A, (M, K), torch.int8, A.device)
+    ldw = _rows(name, "W", W, (N, K), torch.int8, A.device)
+    pa = _flat(name, "scale_a", scale_a, (M,), torch.float32, A.device)
+    pw = _flat(name, "scale_w", scale_w, (N,), torch.float32, A.device)
+    pb = _flat(name, "bias", bias, (N,), torch.float32, A.device)
+    out = _new((M, N), dtype, A.device, stream) if out is None else out
+    ldc = _rows(name, "out", out, (M, N), dtype, A.device)
+    context(d).call("ki_gemm_i8", A.data_ptr(), lda, W.data_ptr(), ldw, pa, pw, pb, code, out.data_ptr(), ldc, M, N, K,
+                    _stream_ptr(stream, d))
+    return out
+
+
+def causal_conv(x, weight, bias=None, state=None, offsets=None, slots=None, initial=None, activation=None, out=None,
+                stream=None):
+    """Causal depthwise convolution of packed sequences: out[t, d] = act(bias[d] + sum_j weight[d, j] *
+    x[t - (width-1) + j, d]) for ``x`` (tokens x channels, contiguous rows) and ``weight`` (channels x width,
+    width 2 to 8), all of one type (Float32, Float16, BFloat16); activation None or 'silu'.
+
+    ``offsets`` (int32, sequences + 1): sequence i holds rows offsets[i] to offsets[i+1]; None: one sequence.
+    ``state`` (slots x (width-1) x channels, x's type): the last inputs of each sequence, oldest first, read
+    before its first row and replaced; sequence i uses slot ``slots[i]`` (int32; None: slot i), negative
+    numbers mark padding that is skipped, and no slot is named twice.  ``initial`` (bool or uint8): False
+    starts the sequence from zeros.  Without a state every sequence starts from zeros.  A bad offset or slot
+    number is reported by ``Context.check``."""
+    name = "causal_conv"
+    d = _dev(x)
+    tokens, channels = _matrix(name, "x", x)
+    _, width = _matrix(name, "weight", weight)
+    code, dev = _float_code(name, x.dtype), x.device
+    ldx = _rows(name, "x", x, (tokens, channels), x.dtype, dev)
+    pw = _flat(name, "weight", weight, (channels, width), x.dtype, dev)
+    pb = _flat(name, "bias", bias, (channels,), x.dtype, dev)
+    count, at, flags = _sequences(name, offsets, initial, state, dev)
+    ps, state_ld, n, pslots = _state(name, state, (width - 1, channels), x.dtype, dev, slots, count)
+    silu = _silu(name, activation)
+    out = _new((tokens, channels), x.dtype, dev, stream) if out is None else out
+    ldy = _rows(name, "out", out, (tokens, channels), x.dtype, dev)
+    context(d).call("ki_causal_conv", code, x.data_ptr(), ldx, pw, pb, ps, state_ld, n, pslots, flags, at, count,
+                    out.data_ptr(), ldy, tokens, channels, width, silu, _stream_ptr(stream, d))
+    return out
+
+
+def causal_conv_step(x, weight, bias=None, state=None, slots=None, activation=None, out=None, stream=None):
+    """One token per row: row r of ``x`` (rows x channels) continues state slot ``slots[r]`` (None: slot r), which
+    is updated; the arguments are those of ``causal_conv``."""
+    name = "causal_conv_step"
+    d = _dev(x)
+    rows, channels = _matrix(name, "x", x)
+    _, width = _matrix(name, "weight", weight)
+    code, dev = _float_code(name, x.dtype), x.device
+    if state is None:
+        raise _bad(f"{name}: a state is needed")
+    ldx = _rows(name, "x", x, (rows, channels), x.dtype, dev)
+    pw = _flat(name, "weight", weight, (channels, width), x.dtype, dev)
+    pb = _flat(name, "bias", bias, (channels,), x.dtype, dev)
+    ps, state_ld, n, pslots = _state(name, state, (width - 1, channels), x.dtype, dev, slots, rows)
+    silu = _silu(name, activation)
+    out = _new((rows, channels), x.dtype, dev, stream) if out is None else out
+    ldy = _rows(name, "out", out, (rows, channels), x.dtype, dev)
+    context(d).call("ki_causal_conv_step", code, x.data_ptr(), ldx, pw, pb, ps, state_ld, n, pslots, out.data_ptr(), ldy,
+                    rows, channels, width, silu, _stream_ptr(stream, d))
+    return out
+
+
+def _per_state(name: str, what: str, t, rows: int, states: int, dtype, device) -> tuple:
+    """(row stride, groups) of B or C: rows x states, or rows x groups x states with contiguous rows."""
+    if t.dim() == 3:
+        groups = t.shape[1]
+        if groups > 1 and states and t.stride(1) != states:
+            raise _bad(f"{name}: {what} must have contiguous rows")
+        if t.device != device or t.dtype != dtype or tuple(t.shape) != (rows, groups, states):
+            raise _bad(f"{name}: {what} must be {dtype} [{rows}, groups, {states}] on {device}")
+        if (states > 1 and t.stride(2) != 1) or (rows > 1 and t.stride(0) < groups * states):
+            raise _bad(f"{name}: {what} must have contiguous rows that do not overlap")
+        return (t.stride(0) if rows > 1 else groups * states), groups
+    if t.dim() != 2:
+        raise _bad(f"{name}: {what} must be 2-D or 3-D")
+    return _rows(name, what, t, (rows, states), dtype, device), 1
+
+
+def _scan_args(name, u, delta, A, B, C, D, z, delta_bias):
+    torch = _torch()
+    rows, channels = _matrix(name, "u", u)
+    _, states = _matrix(name, "A", A)
+    code, dev = _float_code(name, u.dtype), u.device
+    ldu = _rows(name, "u", u, (rows, channels), u.dtype, dev)
+    ldd = _rows(name, "delta", delta, (rows, channels), u.dtype, dev)
+    pA = _flat(name, "A", A, (channels, states), torch.float32, dev)
+    ldb, groups = _per_state(name, "B", B, rows, states, u.dtype, dev)
+    ldc, groups_c = _per_state(name, "C", C, rows, states, u.dtype, dev)
+    if groups != groups_c or groups < 1 or channels % groups:
+        raise _bad(f"{name}: B and C need the same number of groups, a divisor of the channels")
+    pD = _flat(name, "D", D, (channels,), torch.float32, dev)
+    pbias = _flat(name, "delta_bias", delta_bias, (channels,), torch.float32, dev)
+    ldz = 0 if z is None else _rows(name, "z", z, (rows, channels), u.dtype, dev)
+    return rows, channels, states, groups, (code, u.data_ptr(), ldu, delta.data_ptr(), ldd, pA, B.data_ptr(), ldb,
+                                            C.data_ptr(), ldc, pD, None if z is None else z.data_ptr(), ldz, pbias)
+
+
+def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=False, state=None, offsets=None,
+                   slots=None, initial=None, out=None, stream=None):
+    """Selective state space scan of packed sequences.  With s = delta + delta_bias (softplus'd if asked):
+
+        h_t[d, n] = exp(s[t, d] A[d, n]) h_{t-1}[d, n] + s[t, d] u[t, d] B[t, g, n]
+        out[t, d] = (sum_n C[t, g, n] h_t[d, n] + D[d] u[t, d]) * z[t, d] sigmoid(z[t, d])
+
+    ``u``, ``delta``, ``z``: tokens x channels; ``B``, ``C``: tokens x states, or tokens x groups x states (channel d
+    belongs to group d // (channels / groups)), all of one type (Float32, Float16, BFloat16) with contiguous
+    rows; ``A``: channels x states, ``D``, ``delta_bias``: channels, Float32.  D, z and delta_bias may be None.
+    ``state``: Float32 slots x channels x states; it, ``offsets``, ``slots`` and ``initial`` are as in ``causal_conv``."""
+    torch = _torch()
+    name = "selective_scan"
+    d = _dev(u)
+    rows, channels, states, groups, args = _scan_args(name, u, delta, A, B, C, D, z, delta_bias)
+    count, at, flags = _sequences(name, offsets, initial, state, u.device)
+    ps, state_ld, n, pslots = _state(name, state, (channels, states), torch.float32, u.device, slots, count)
+    out = _new((rows, channels), u.dtype, u.device, stream) if out is None else out
+    ldy = _rows(name, "out", out, (rows, channels), u.dtype, u.device)
+    context(d).call("ki_selective_scan", *args, int(bool(softplus)), ps, state_ld, n, pslots, flags, at, count,
+                    out.data_ptr(), ldy, rows, channels, states, groups, _stream_ptr(stream, d))
+    return out
+
+
+def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=False, state=None, slots=None,
+                        out=None, stream=None):
+    """One token per row: row r of ``u`` (rows x channels) continues state slot ``slots[r]`` (None: slot r), which
+    is updated; the arguments are those of ``selective_scan``."""
+    torch = _torch()
+    name = "selective_scan_step"
+    d = _dev(u)
+    rows, channels, states, groups, args = _scan_args(name, u, delta, A, B, C, D, z, delta_bias)
+    if state is None:
+        raise _bad(f"{name}: a state is needed")
+    ps, state_ld, n, pslots = _state(name, state, (channels, states), torch.float32, u.device, slots, rows)
+    out = _new((rows, channels), u.dtype, u.device, stream) if out is None else out
+    ldy = _rows(name, "out", out, (rows, channels), u.dtype, u.device)
+    context(d).call("ki_selective_scan_step", *args, int(bool(softplus)), ps, state_ld, n, pslots, out.data_ptr(), ldy,
+                    rows, channels, states, groups, _stream_ptr(stream, d))
+    return out
 
 
 # ---------------------------------------------------------------------------------------------

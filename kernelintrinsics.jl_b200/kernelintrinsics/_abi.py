@@ -25,6 +25,7 @@ DIR = {"up": 0, "down": 1, "xor": 2, "idx": 3}
 MODE = {"all": 0, "any": 1, "uni": 2, "ballot": 3}
 DTYPE = {"int8": 0, "uint8": 1, "int16": 2, "uint16": 3, "int32": 4, "uint32": 5, "int64": 6, "uint64": 7,
          "float32": 8, "float64": 9}
+FLOAT_DTYPE = {"float32": 8, "float16": 10, "bfloat16": 11}  # element types of a layer's operators
 OP = {"+": 0, "max": 1, "min": 2, "|": 3, "&": 4, "^": 5}
 
 # Every symbol the header declares, with (restype, argtypes).
@@ -74,6 +75,16 @@ SIGNATURES = {
     "ki_scan_inclusive_i64_noalloc": (_i32, [_vp, _vp, _sz, _i64, _vp]),
     "ki_compact_gt_f32": (_i32, [_vp, _vp, _sz, _f32, _vp, _vp, _i64, _vp, _vp]),
     "ki_gemm_e4m3_f32": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _f32, _f32, _vp]),
+    "ki_quantize_rows": (_i32, [_vp, _i32, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp]),
+    "ki_gemm_i8": (_i32, [_vp, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _i32, _vp, _sz, _sz, _sz, _sz, _vp]),
+    "ki_causal_conv": (_i32, [_vp, _i32, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz,
+                              _i32, _i32, _vp]),
+    "ki_causal_conv_step": (_i32, [_vp, _i32, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _sz, _sz, _sz, _i32, _i32,
+                                   _vp]),
+    "ki_selective_scan": (_i32, [_vp, _i32, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _i32, _vp,
+                                 _sz, _sz, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz, _vp]),
+    "ki_selective_scan_step": (_i32, [_vp, _i32, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _i32,
+                                      _vp, _sz, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _vp]),
     "ki_warp_shfl": (_i32, [_vp, _i32, _vp, _vp, _sz, _sz, _i32, _vp]),
     "ki_warp_reduce": (_i32, [_vp, _i32, _i32, _vp, _vp, _sz, _vp]),
     "ki_warp_fold": (_i32, [_vp, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
