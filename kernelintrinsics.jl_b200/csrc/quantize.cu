@@ -1,8 +1,9 @@
 // quantize.cu -- ki_quantize_rows: rows of Float32 / Float16 / BFloat16 to int8 with one scale per row.
 //
-//   scale[r] = max_c |x[r, c]| / 127,   q[r, c] = rint(x[r, c] / scale[r]), ties to even, in [-127, 127]
+//   scale[r] = max_c |x[r, c]| * (1 / 127),   q[r, c] = rint(x[r, c] / scale[r]), ties to even, in [-127, 127]
 //
-// Both quotients are IEEE Float32, so the int8 values are defined bit for bit.  A row of zeros (or one
+// The product (with 1 / 127 as a Float32) and the quotient are IEEE Float32, so the int8 values are
+// defined bit for bit.  A row of zeros (or one
 // whose scale underflows to zero) gives zeros; a NaN or an infinity makes the row's scale NaN or
 // infinite and q zero where x / scale is NaN or zero, so that a product with the row shows NaN.
 //
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(TPR > kThreads ? TPR : kThreads)
         for (int i = 0; i < kRowWarps; ++i) m = max(m, part[w0 + i]);
     }
     if (!live) return;
-    const float s = __fdiv_rn(__uint_as_float(m), 127.0f);
+    const float s = __uint_as_float(m) * (1.0f / 127.0f);
     const bool zero = s == 0.0f;
     const float inv = zero ? 0.0f : __fdiv_rn(1.0f, s);
     if (t == 0) scale[r] = s;

@@ -132,10 +132,16 @@ class Ballot(Mode):
 # ---------------------------------------------------------------------------------------------
 # context
 # ---------------------------------------------------------------------------------------------
-def _torch():
-    import torch
+_torch_module = None
 
-    return torch
+
+def _torch():
+    global _torch_module
+    if _torch_module is None:
+        import torch
+
+        _torch_module = torch
+    return _torch_module
 
 
 class Context:
@@ -775,116 +781,147 @@ def fp8_gemm(A, B, C=None, scale_a: float = 1.0, scale_b: float = 1.0, stream=No
 
 
 # ---------------------------------------------------------------------------------------------
-# operators of a state-space layer served in 8 bits
+# operators of a state-space layer served in 8 bits.  Single-token calls take less time on the GPU
+# than in Python, so these checks read each tensor's properties once and build messages only to raise.
 # ---------------------------------------------------------------------------------------------
+_float_codes: dict = {}
+
+
 def _bad(what: str):
     return KIArgumentError(_abi.KI_ERR_ARG, what)
 
 
 def _float_code(name: str, dtype) -> int:
-    code = _abi.FLOAT_DTYPE.get(str(dtype)[6:])
+    if not _float_codes:
+        _float_codes.update({getattr(_torch(), k): v for k, v in _abi.FLOAT_DTYPE.items()})
+    code = _float_codes.get(dtype)
     if code is None:
         raise _bad(f"{name}: float32, float16 or bfloat16 elements, not {dtype}")
     return code
 
 
-def _rows(name: str, what: str, t, shape: tuple, dtype, device) -> int:
-    """The row stride of a 2-D ``t`` of this shape, type and device whose rows are contiguous."""
-    if t.device != device:
-        raise _bad(f"{name}: {what} is on {t.device}, the first argument on {device}")
-    if t.dtype != dtype or tuple(t.shape) != shape:
+def _refuse(name: str, what: str, t, shape: tuple, dtype, d: int, how: str):
+    if t.get_device() != d:
+        raise _bad(f"{name}: {what} is on {t.device}, not on cuda:{d}")
+    if t.dtype != dtype or t.shape != shape:
         raise _bad(f"{name}: {what} must be {dtype} {list(shape)}, not {t.dtype} {list(t.shape)}")
+    raise _bad(f"{name}: {what} must {how}")
+
+
+def _rows(name: str, what: str, t, shape: tuple, dtype, d: int) -> int:
+    """The row stride of a 2-D ``t`` of this shape and type on device ``d`` whose rows are contiguous."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != d:
+        _refuse(name, what, t, shape, dtype, d, "")
+    rows, cols = shape
     ld, inner = t.stride()
-    if (shape[1] > 1 and inner != 1) or (shape[0] > 1 and ld < shape[1]):
-        raise _bad(f"{name}: {what} must have contiguous rows that do not overlap")
-    return ld if shape[0] > 1 else shape[1]
+    if (inner != 1 and cols > 1) or (ld < cols and rows > 1):
+        _refuse(name, what, t, shape, dtype, d, "have contiguous rows that do not overlap")
+    return ld if rows > 1 else cols
 
 
-def _flat(name: str, what: str, t, shape: tuple, dtype, device):
-    """A pointer to ``t``, contiguous and of this shape, type and device; None stays None."""
+def _flat(name: str, what: str, t, shape: tuple, dtype, d: int):
+    """A pointer to ``t``, contiguous, of this shape and type and on device ``d``; None stays None."""
     if t is None:
         return None
-    if t.device != device or t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-        raise _bad(f"{name}: {what} must be {dtype} {list(shape)}, contiguous and on {device}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != d or not t.is_contiguous():
+        _refuse(name, what, t, shape, dtype, d, "be contiguous")
     return t.data_ptr()
 
 
-def _new(shape, dtype, device, stream):
-    """An output that belongs to the stream that writes it."""
-    torch = _torch()
+def _new(shape: tuple, dtype, like, stream):
+    """A new tensor on ``like``'s device that belongs to the stream that writes it."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
+    with _torch().cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
 
 
-def _state(name: str, state, inner: tuple, dtype, device, slots, count: int):
+def _raw_stream(stream, d: int) -> int:
+    if stream is not None:
+        if stream.device.index != d:
+            raise _bad(f"stream of cuda:{stream.device.index} for tensors on cuda:{d}")
+        return stream.cuda_stream
+    return _torch()._C._cuda_getCurrentRawStream(d)
+
+
+def _state(name: str, state, first: int, second: int, dtype, d: int, slots, count: int):
     """(pointer, elements between slots, slots, pointer to the slot numbers) of a cache of states."""
-    torch = _torch()
     if state is None:
         if slots is not None:
             raise _bad(f"{name}: slots without a state")
         return None, 0, 0, None
-    if state.device != device or state.dtype != dtype or state.dim() != 3 or tuple(state.shape[1:]) != inner:
-        raise _bad(f"{name}: state must be {dtype} [slots, {inner[0]}, {inner[1]}] on {device}")
-    n, held = state.shape[0], inner[0] * inner[1]
-    if held and n and not state[0].is_contiguous():
-        raise _bad(f"{name}: every slot of the state must be contiguous")
-    ld = state.stride(0) if n > 1 else held
-    if ld < held:
-        raise _bad(f"{name}: slots of the state overlap")
-    if slots is None and n < count:
-        raise _bad(f"{name}: {n} state slots for {count} sequences")
-    return state.data_ptr(), ld, n, _flat(name, "slots", slots, (count,), torch.int32, device)
+    if state.dtype is not dtype or state.dim() != 3 or state.shape[1:] != (first, second) or state.get_device() != d:
+        raise _bad(f"{name}: state must be {dtype} [slots, {first}, {second}] on cuda:{d}")
+    n, held = state.shape[0], first * second
+    ld = held
+    if not state.is_contiguous():
+        ld, mid, inner = state.stride()
+        if (inner != 1 and second > 1) or (mid != second and first > 1):
+            raise _bad(f"{name}: every slot of the state must be contiguous")
+        if n <= 1:
+            ld = held
+        elif ld < held:
+            raise _bad(f"{name}: slots of the state overlap")
+    if slots is None:
+        if n < count:
+            raise _bad(f"{name}: {n} state slots for {count} sequences")
+        return state.data_ptr(), ld, n, None
+    return state.data_ptr(), ld, n, _flat(name, "slots", slots, (count,), _torch().int32, d)
 
 
-def _sequences(name: str, offsets, initial, state, device):
+def _sequences(name: str, offsets, initial, state, d: int):
     """(sequences, pointer to the offsets, pointer to the initial flags)."""
     torch = _torch()
-    if offsets is None:
-        count = 1
-    else:
-        if offsets.dim() != 1 or offsets.numel() < 1:
+    count = 1
+    if offsets is not None:
+        if offsets.dim() != 1 or offsets.shape[0] < 1:
             raise _bad(f"{name}: offsets must hold one value more than there are sequences")
-        count = offsets.numel() - 1
-    at = _flat(name, "offsets", offsets, (count + 1,), torch.int32, device)
+        count = offsets.shape[0] - 1
+    at = _flat(name, "offsets", offsets, (count + 1,), torch.int32, d)
     if initial is not None:
         if state is None:
             raise _bad(f"{name}: initial without a state")
         if initial.dtype not in (torch.bool, torch.uint8):
             raise _bad(f"{name}: initial must be bool or uint8")
-        initial = _flat(name, "initial", initial, (count,), initial.dtype, device)
+        initial = _flat(name, "initial", initial, (count,), initial.dtype, d)
     return count, at, initial
 
 
 def _silu(name: str, activation) -> int:
-    if activation not in (None, "silu"):
+    if activation is None:
+        return 0
+    if activation != "silu":
         raise _bad(f"{name}: activation must be 'silu' or None")
-    return int(activation == "silu")
+    return 1
 
 
 def _matrix(name: str, what: str, t) -> tuple:
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         raise _bad(f"{name}: {what} must be 2-D")
-    return tuple(t.shape)
+    return shape
 
 
 def quantize_rows(x, out=None, scale=None, stream=None):
-    """int8 rows with one scale each: scale[r] = max|x[r]| / 127, out[r] = rint(x[r] / scale[r]) (ties to
-    even, both quotients in Float32), for a 2-D Float32, Float16 or BFloat16 ``x`` with contiguous rows.
+    """int8 rows with one scale each: scale[r] = max|x[r]| * (1 / 127), out[r] = rint(x[r] / scale[r]) (ties
+    to even, all in Float32), for a 2-D Float32, Float16 or BFloat16 ``x`` with contiguous rows.
     A row of zeros gives zeros and scale 0; a NaN or an infinity stays in the row's scale.
     Returns (out, scale): int8 of x's shape, Float32 per row."""
     torch = _torch()
+    name = "quantize_rows"
     d = _dev(x)
-    rows, cols = _matrix("quantize_rows", "x", x)
-    code = _float_code("quantize_rows", x.dtype)
-    ld = _rows("quantize_rows", "x", x, (rows, cols), x.dtype, x.device)
-    out = _new((rows, cols), torch.int8, x.device, stream) if out is None else out
-    scale = _new((rows,), torch.float32, x.device, stream) if scale is None else scale
-    ldq = _rows("quantize_rows", "out", out, (rows, cols), torch.int8, x.device)
-    ps = _flat("quantize_rows", "scale", scale, (rows,), torch.float32, x.device)
+    rows, cols = shape = _matrix(name, "x", x)
+    code = _float_code(name, x.dtype)
+    ld = _rows(name, "x", x, shape, x.dtype, d)
+    if out is None:
+        out, ldq = _new(shape, torch.int8, x, stream), cols
+    else:
+        ldq = _rows(name, "out", out, shape, torch.int8, d)
+    if scale is None:
+        scale = _new((rows,), torch.float32, x, stream)
+    ps = _flat(name, "scale", scale, (rows,), torch.float32, d)
     context(d).call("ki_quantize_rows", code, x.data_ptr(), rows, cols, ld, out.data_ptr(), ldq, ps,
-                    _stream_ptr(stream, d))
+                    _raw_stream(stream, d))
     return out, scale
 
 
@@ -895,21 +932,23 @@ def int8_gemm(A, W, scale_a, scale_w, bias=None, out=None, dtype=None, stream=No
     torch = _torch()
     name = "int8_gemm"
     d = _dev(A)
-    (M, K), (N, KW) = _matrix(name, "A", A), _matrix(name, "W", W)
-    if K != KW:
-        raise _bad(f"{name}: inner dimensions differ")
+    M, K = shape = _matrix(name, "A", A)
+    N = _matrix(name, "W", W)[0]
     if dtype is None:
         dtype = torch.bfloat16 if out is None else out.dtype
     code = _float_code(name, dtype)
-    lda = _rows(name, "A", A, (M, K), torch.int8, A.device)
-    ldw = _rows(name, "W", W, (N, K), torch.int8, A.device)
-    pa = _flat(name, "scale_a", scale_a, (M,), torch.float32, A.device)
-    pw = _flat(name, "scale_w", scale_w, (N,), torch.float32, A.device)
-    pb = _flat(name, "bias", bias, (N,), torch.float32, A.device)
-    out = _new((M, N), dtype, A.device, stream) if out is None else out
-    ldc = _rows(name, "out", out, (M, N), dtype, A.device)
+    lda = _rows(name, "A", A, shape, torch.int8, d)
+    ldw = _rows(name, "W", W, (N, K), torch.int8, d)
+    f32 = torch.float32
+    pa = _flat(name, "scale_a", scale_a, (M,), f32, d)
+    pw = _flat(name, "scale_w", scale_w, (N,), f32, d)
+    pb = _flat(name, "bias", bias, (N,), f32, d)
+    if out is None:
+        out, ldc = _new((M, N), dtype, A, stream), N
+    else:
+        ldc = _rows(name, "out", out, (M, N), dtype, d)
     context(d).call("ki_gemm_i8", A.data_ptr(), lda, W.data_ptr(), ldw, pa, pw, pb, code, out.data_ptr(), ldc, M, N, K,
-                    _stream_ptr(stream, d))
+                    _raw_stream(stream, d))
     return out
 
 
@@ -923,23 +962,27 @@ def causal_conv(x, weight, bias=None, state=None, offsets=None, slots=None, init
     ``state`` (slots x (width-1) x channels, x's type): the last inputs of each sequence, oldest first, read
     before its first row and replaced; sequence i uses slot ``slots[i]`` (int32; None: slot i), negative
     numbers mark padding that is skipped, and no slot is named twice.  ``initial`` (bool or uint8): False
-    starts the sequence from zeros.  Without a state every sequence starts from zeros.  A bad offset or slot
-    number is reported by ``Context.check``."""
+    starts the sequence from zeros.  Without a state every sequence starts from zeros.  Rows of no sequence
+    are not written (a new output holds anything there).  A bad offset or slot number is reported by
+    ``Context.check``."""
     name = "causal_conv"
     d = _dev(x)
-    tokens, channels = _matrix(name, "x", x)
-    _, width = _matrix(name, "weight", weight)
-    code, dev = _float_code(name, x.dtype), x.device
-    ldx = _rows(name, "x", x, (tokens, channels), x.dtype, dev)
-    pw = _flat(name, "weight", weight, (channels, width), x.dtype, dev)
-    pb = _flat(name, "bias", bias, (channels,), x.dtype, dev)
-    count, at, flags = _sequences(name, offsets, initial, state, dev)
-    ps, state_ld, n, pslots = _state(name, state, (width - 1, channels), x.dtype, dev, slots, count)
+    tokens, channels = shape = _matrix(name, "x", x)
+    width = _matrix(name, "weight", weight)[1]
+    dtype = x.dtype
+    code = _float_code(name, dtype)
+    ldx = _rows(name, "x", x, shape, dtype, d)
+    pw = _flat(name, "weight", weight, (channels, width), dtype, d)
+    pb = _flat(name, "bias", bias, (channels,), dtype, d)
+    count, at, flags = _sequences(name, offsets, initial, state, d)
+    ps, state_ld, n, pslots = _state(name, state, width - 1, channels, dtype, d, slots, count)
     silu = _silu(name, activation)
-    out = _new((tokens, channels), x.dtype, dev, stream) if out is None else out
-    ldy = _rows(name, "out", out, (tokens, channels), x.dtype, dev)
+    if out is None:
+        out, ldy = _new(shape, dtype, x, stream), channels
+    else:
+        ldy = _rows(name, "out", out, shape, dtype, d)
     context(d).call("ki_causal_conv", code, x.data_ptr(), ldx, pw, pb, ps, state_ld, n, pslots, flags, at, count,
-                    out.data_ptr(), ldy, tokens, channels, width, silu, _stream_ptr(stream, d))
+                    out.data_ptr(), ldy, tokens, channels, width, silu, _raw_stream(stream, d))
     return out
 
 
@@ -948,56 +991,60 @@ def causal_conv_step(x, weight, bias=None, state=None, slots=None, activation=No
     is updated; the arguments are those of ``causal_conv``."""
     name = "causal_conv_step"
     d = _dev(x)
-    rows, channels = _matrix(name, "x", x)
-    _, width = _matrix(name, "weight", weight)
-    code, dev = _float_code(name, x.dtype), x.device
+    rows, channels = shape = _matrix(name, "x", x)
+    width = _matrix(name, "weight", weight)[1]
+    dtype = x.dtype
+    code = _float_code(name, dtype)
     if state is None:
         raise _bad(f"{name}: a state is needed")
-    ldx = _rows(name, "x", x, (rows, channels), x.dtype, dev)
-    pw = _flat(name, "weight", weight, (channels, width), x.dtype, dev)
-    pb = _flat(name, "bias", bias, (channels,), x.dtype, dev)
-    ps, state_ld, n, pslots = _state(name, state, (width - 1, channels), x.dtype, dev, slots, rows)
+    ldx = _rows(name, "x", x, shape, dtype, d)
+    pw = _flat(name, "weight", weight, (channels, width), dtype, d)
+    pb = _flat(name, "bias", bias, (channels,), dtype, d)
+    ps, state_ld, n, pslots = _state(name, state, width - 1, channels, dtype, d, slots, rows)
     silu = _silu(name, activation)
-    out = _new((rows, channels), x.dtype, dev, stream) if out is None else out
-    ldy = _rows(name, "out", out, (rows, channels), x.dtype, dev)
+    if out is None:
+        out, ldy = _new(shape, dtype, x, stream), channels
+    else:
+        ldy = _rows(name, "out", out, shape, dtype, d)
     context(d).call("ki_causal_conv_step", code, x.data_ptr(), ldx, pw, pb, ps, state_ld, n, pslots, out.data_ptr(), ldy,
-                    rows, channels, width, silu, _stream_ptr(stream, d))
+                    rows, channels, width, silu, _raw_stream(stream, d))
     return out
 
 
-def _per_state(name: str, what: str, t, rows: int, states: int, dtype, device) -> tuple:
+def _per_state(name: str, what: str, t, rows: int, states: int, dtype, d: int) -> tuple:
     """(row stride, groups) of B or C: rows x states, or rows x groups x states with contiguous rows."""
-    if t.dim() == 3:
-        groups = t.shape[1]
-        if groups > 1 and states and t.stride(1) != states:
-            raise _bad(f"{name}: {what} must have contiguous rows")
-        if t.device != device or t.dtype != dtype or tuple(t.shape) != (rows, groups, states):
-            raise _bad(f"{name}: {what} must be {dtype} [{rows}, groups, {states}] on {device}")
-        if (states > 1 and t.stride(2) != 1) or (rows > 1 and t.stride(0) < groups * states):
-            raise _bad(f"{name}: {what} must have contiguous rows that do not overlap")
-        return (t.stride(0) if rows > 1 else groups * states), groups
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) == 2:
+        return _rows(name, what, t, (rows, states), dtype, d), 1
+    if len(shape) != 3:
         raise _bad(f"{name}: {what} must be 2-D or 3-D")
-    return _rows(name, what, t, (rows, states), dtype, device), 1
+    groups = shape[1]
+    if t.dtype is not dtype or shape[0] != rows or shape[2] != states or t.get_device() != d:
+        _refuse(name, what, t, (rows, groups, states), dtype, d, "")
+    ld, mid, inner = t.stride()
+    if (inner != 1 and states > 1) or (mid != states and groups > 1) or (ld < groups * states and rows > 1):
+        _refuse(name, what, t, shape, dtype, d, "have contiguous rows that do not overlap")
+    return (ld if rows > 1 else groups * states), groups
 
 
-def _scan_args(name, u, delta, A, B, C, D, z, delta_bias):
-    torch = _torch()
-    rows, channels = _matrix(name, "u", u)
-    _, states = _matrix(name, "A", A)
-    code, dev = _float_code(name, u.dtype), u.device
-    ldu = _rows(name, "u", u, (rows, channels), u.dtype, dev)
-    ldd = _rows(name, "delta", delta, (rows, channels), u.dtype, dev)
-    pA = _flat(name, "A", A, (channels, states), torch.float32, dev)
-    ldb, groups = _per_state(name, "B", B, rows, states, u.dtype, dev)
-    ldc, groups_c = _per_state(name, "C", C, rows, states, u.dtype, dev)
+def _scan_args(name, u, delta, A, B, C, D, z, delta_bias, d):
+    f32 = _torch().float32
+    rows, channels = shape = _matrix(name, "u", u)
+    states = _matrix(name, "A", A)[1]
+    dtype = u.dtype
+    code = _float_code(name, dtype)
+    ldu = _rows(name, "u", u, shape, dtype, d)
+    ldd = _rows(name, "delta", delta, shape, dtype, d)
+    pA = _flat(name, "A", A, (channels, states), f32, d)
+    ldb, groups = _per_state(name, "B", B, rows, states, dtype, d)
+    ldc, groups_c = _per_state(name, "C", C, rows, states, dtype, d)
     if groups != groups_c or groups < 1 or channels % groups:
         raise _bad(f"{name}: B and C need the same number of groups, a divisor of the channels")
-    pD = _flat(name, "D", D, (channels,), torch.float32, dev)
-    pbias = _flat(name, "delta_bias", delta_bias, (channels,), torch.float32, dev)
-    ldz = 0 if z is None else _rows(name, "z", z, (rows, channels), u.dtype, dev)
-    return rows, channels, states, groups, (code, u.data_ptr(), ldu, delta.data_ptr(), ldd, pA, B.data_ptr(), ldb,
-                                            C.data_ptr(), ldc, pD, None if z is None else z.data_ptr(), ldz, pbias)
+    pD = _flat(name, "D", D, (channels,), f32, d)
+    pbias = _flat(name, "delta_bias", delta_bias, (channels,), f32, d)
+    ldz, pz = (0, None) if z is None else (_rows(name, "z", z, shape, dtype, d), z.data_ptr())
+    return shape, states, groups, (code, u.data_ptr(), ldu, delta.data_ptr(), ldd, pA, B.data_ptr(), ldb, C.data_ptr(),
+                                   ldc, pD, pz, ldz, pbias)
 
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=False, state=None, offsets=None,
@@ -1011,16 +1058,18 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     belongs to group d // (channels / groups)), all of one type (Float32, Float16, BFloat16) with contiguous
     rows; ``A``: channels x states, ``D``, ``delta_bias``: channels, Float32.  D, z and delta_bias may be None.
     ``state``: Float32 slots x channels x states; it, ``offsets``, ``slots`` and ``initial`` are as in ``causal_conv``."""
-    torch = _torch()
     name = "selective_scan"
     d = _dev(u)
-    rows, channels, states, groups, args = _scan_args(name, u, delta, A, B, C, D, z, delta_bias)
-    count, at, flags = _sequences(name, offsets, initial, state, u.device)
-    ps, state_ld, n, pslots = _state(name, state, (channels, states), torch.float32, u.device, slots, count)
-    out = _new((rows, channels), u.dtype, u.device, stream) if out is None else out
-    ldy = _rows(name, "out", out, (rows, channels), u.dtype, u.device)
-    context(d).call("ki_selective_scan", *args, int(bool(softplus)), ps, state_ld, n, pslots, flags, at, count,
-                    out.data_ptr(), ldy, rows, channels, states, groups, _stream_ptr(stream, d))
+    shape, states, groups, args = _scan_args(name, u, delta, A, B, C, D, z, delta_bias, d)
+    rows, channels = shape
+    count, at, flags = _sequences(name, offsets, initial, state, d)
+    ps, state_ld, n, pslots = _state(name, state, channels, states, _torch().float32, d, slots, count)
+    if out is None:
+        out, ldy = _new(shape, u.dtype, u, stream), channels
+    else:
+        ldy = _rows(name, "out", out, shape, u.dtype, d)
+    context(d).call("ki_selective_scan", *args, 1 if softplus else 0, ps, state_ld, n, pslots, flags, at, count,
+                    out.data_ptr(), ldy, rows, channels, states, groups, _raw_stream(stream, d))
     return out
 
 
@@ -1028,17 +1077,19 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, soft
                         out=None, stream=None):
     """One token per row: row r of ``u`` (rows x channels) continues state slot ``slots[r]`` (None: slot r), which
     is updated; the arguments are those of ``selective_scan``."""
-    torch = _torch()
     name = "selective_scan_step"
     d = _dev(u)
-    rows, channels, states, groups, args = _scan_args(name, u, delta, A, B, C, D, z, delta_bias)
+    shape, states, groups, args = _scan_args(name, u, delta, A, B, C, D, z, delta_bias, d)
+    rows, channels = shape
     if state is None:
         raise _bad(f"{name}: a state is needed")
-    ps, state_ld, n, pslots = _state(name, state, (channels, states), torch.float32, u.device, slots, rows)
-    out = _new((rows, channels), u.dtype, u.device, stream) if out is None else out
-    ldy = _rows(name, "out", out, (rows, channels), u.dtype, u.device)
-    context(d).call("ki_selective_scan_step", *args, int(bool(softplus)), ps, state_ld, n, pslots, out.data_ptr(), ldy,
-                    rows, channels, states, groups, _stream_ptr(stream, d))
+    ps, state_ld, n, pslots = _state(name, state, channels, states, _torch().float32, d, slots, rows)
+    if out is None:
+        out, ldy = _new(shape, u.dtype, u, stream), channels
+    else:
+        ldy = _rows(name, "out", out, shape, u.dtype, d)
+    context(d).call("ki_selective_scan_step", *args, 1 if softplus else 0, ps, state_ld, n, pslots, out.data_ptr(), ldy,
+                    rows, channels, states, groups, _raw_stream(stream, d))
     return out
 
 

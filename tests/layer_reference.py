@@ -93,12 +93,12 @@ def scan(u, delta, A, B, C, D, z, delta_bias, soft, spans, states):
 
 
 def quantize(x):
-    """scale and int8 of Float32 rows, by IEEE Float32 division as the operator is defined (bit for bit)."""
+    """scale and int8 of Float32 rows, by IEEE Float32 operations as the operator is defined (bit for bit)."""
     x = x.astype(np.float32)
     bits = np.abs(x).view(np.uint32)
     top = bits.max(1).view(np.float32) if x.shape[1] else np.zeros(x.shape[0], np.float32)
     with np.errstate(all="ignore"):
-        scale = (top / np.float32(127)).astype(np.float32)
+        scale = (top * (np.float32(1) / np.float32(127))).astype(np.float32)
         q = np.rint((x / scale[:, None]).astype(np.float32))
         q = np.where(np.isnan(q) | (scale[:, None] == 0), 0, np.clip(q, -127, 127))
     return scale, q.astype(np.int8)
