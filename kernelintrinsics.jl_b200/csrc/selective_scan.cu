@@ -37,35 +37,235 @@ struct ScanArgs {
     size_t ldy;
     int channels, states, groups;
     bool soft;
+    bool vec;           // rows of u, delta, z and y are aligned for accesses of a thread's channels
+    bool vec_b, vec_c;  // rows of B and C are aligned for accesses of a thread's states
     ki::Sequences seq;
 };
 
-// Folds p[0..L) over the L lanes that share a channel: lane l ends up with the sum of p[l].
-template <int L>
-__device__ __forceinline__ float fold_lanes(float (&p)[L], int lane) {
+constexpr int kTime = 32;      // tokens per chunk
+constexpr int kUnroll = 8;
+constexpr int kLanes = 128;    // threads per block that compute
+constexpr int kHelpers = 128;  // and that load and store
+constexpr int kShare = kHelpers / kTime;  // helper threads that share a token
+
+__device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// N elements of a row, kept as they lie in memory until they are used, so that nothing waits for a load that runs
+// ahead.  `vec`: the row is aligned for whole accesses; n: how many elements exist.
+template <class T, int N>
+struct Raw {
+    static constexpr int BYTES = N * (int)sizeof(T);
+    static constexpr int NW = BYTES < 4 ? 1 : BYTES / 4;
+    uint32_t w[NW];
+
+    __device__ __forceinline__ void load(const T* p, bool vec, int n) {
+        if (vec && n >= N) {
+            if constexpr (BYTES >= 16) {
 #pragma unroll
-    for (int h = L / 2; h >= 1; h /= 2) {
-        const bool up = lane & h;
+                for (int i = 0; i < NW; i += 4) {
+                    const uint4 v = reinterpret_cast<const uint4*>(p)[i / 4];
+                    w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+                }
+            } else if constexpr (BYTES == 8) {
+                const uint2 v = *reinterpret_cast<const uint2*>(p);
+                w[0] = v.x, w[1] = v.y;
+            } else if constexpr (BYTES == 4) {
+                w[0] = *reinterpret_cast<const uint32_t*>(p);
+            } else {
+                w[0] = *reinterpret_cast<const uint16_t*>(p);
+            }
+        } else {
 #pragma unroll
-        for (int i = 0; i < h; ++i) {
-            const float send = up ? p[i] : p[i + h];
-            const float keep = up ? p[i + h] : p[i];
-            p[i] = keep + __shfl_xor_sync(0xffffffffu, send, h);
+            for (int i = 0; i < NW; ++i) w[i] = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i < n) set(i, p[i]);
         }
     }
-    return p[0];
-}
+    __device__ __forceinline__ void store(T* p, bool vec, int n) const {
+        if (vec && n >= N) {
+            if constexpr (BYTES >= 16) {
+#pragma unroll
+                for (int i = 0; i < NW; i += 4)
+                    reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+            } else if constexpr (BYTES == 8) {
+                *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+            } else if constexpr (BYTES == 4) {
+                *reinterpret_cast<uint32_t*>(p) = w[0];
+            } else {
+                *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i < n) p[i] = get(i);
+        }
+    }
+    __device__ __forceinline__ T get(int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[i]);
+        } else {
+            const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+            return *reinterpret_cast<const T*>(&h);
+        }
+    }
+    __device__ __forceinline__ uint32_t half(int i) const { return (w[i / 2] >> (16 * (i & 1))) & 0xffffu; }
+    __device__ __forceinline__ void set(int i, T v) {  // into words that were zero there
+        if constexpr (sizeof(T) == 4)
+            w[i] = __float_as_uint(v);
+        else
+            w[i / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(&v) << (16 * (i & 1));
+    }
+};
 
 template <class T, int LPC, int K>
-__global__ void __launch_bounds__(kThreads) scan_kernel(const ScanArgs a, int tiles) {
-    constexpr int DT = kThreads / LPC;         // channels per block
-    constexpr int NP = LPC * K;                // states, padded
-    constexpr int TC = NP <= 64 ? 64 : 16;     // tokens per chunk
-    __shared__ float2 s_step[TC][DT];          // (s_t, s_t u_t)
-    __shared__ float2 s_bc[TC][NP];
-    __shared__ float s_y[TC][DT + 1];
+struct Tile {
+    static constexpr int DT = kLanes / LPC;         // channels per block
+    static constexpr int VC = DT / kShare;         // channels per helper thread
+    static constexpr int NP = LPC * K;             // states, padded
+    static constexpr int NB = NP / kShare;          // states of B and C per helper thread
+    static constexpr int GW = 2 * K * (int)sizeof(T) / 4;  // words of a lane's states: K of B, then K of C, as loaded
+    static constexpr int ROW = DT + 2;             // of steps, padded so that neighbouring tokens' banks differ
+    struct Stage {
+        float4 part[kTime * kLanes / 4];  // each lane's sum over its states, swizzled
+        uint32_t bc[kTime * LPC * GW];
+        float2 step[kTime * ROW];        // (s, s u) of a token and channel
+    };
+    // 16 bytes number `slot` of a token's sums.  The helper threads of a token and of the next ones read the same
+    // banks at once; the exclusive-or puts eight neighbouring threads on all of them.
+    static __device__ __forceinline__ int part_at(int t, int slot) {
+        return t * (kLanes / 4) + (slot ^ (slot / (kLanes / 4 / kShare) + kShare * (t & (8 / kShare - 1))));
+    }
+};
+
+// Two neighbouring 16-bit values of a word.
+template <class T>
+__device__ __forceinline__ ki::f32x2 widen2(uint32_t w);
+template <>
+__device__ __forceinline__ ki::f32x2 widen2<__nv_bfloat16>(uint32_t w) {
+    return ki::pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ ki::f32x2 widen2<__half>(uint32_t w) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return ki::pair(f.x, f.y);
+}
+
+// Compute threads.  A token passes three stages that run on three tokens at once, so that the exponentials of one
+// (16 a clock and SM) and the multiply-adds of another share the time: its values are loaded, then its decays and
+// what it adds are computed, then the states and the sum over them.
+template <class T, int LPC, int K>
+struct Lane {
+    using L = Tile<T, LPC, K>;
+    static constexpr int GW = L::GW;
+    static constexpr int P = K == 1 ? 1 : K / 2;  // pairs of states (one state: only the first half is used)
+    float A[2 * P], h[2 * P];
+
+    struct In {
+        float2 x;
+        uint32_t w[GW];
+    };
+    struct Mid {
+        ki::f32x2 a[P], add[P], c[P];
+    };
+    static __device__ __forceinline__ In load(const float2* step, const uint32_t* bc, int t) {
+        In in;
+        in.x = step[t * L::ROW];
+        constexpr int W = GW < 4 ? GW : 4;
+#pragma unroll
+        for (int i = 0; i < GW; i += W) {
+            const ki::Vec<uint32_t, W> v = ki::load_vec<uint32_t, W>(bc + t * (LPC * GW) + i);
+#pragma unroll
+            for (int j = 0; j < W; ++j) in.w[i + j] = v.e[j];
+        }
+        return in;
+    }
+    __device__ __forceinline__ Mid decays(const In& in) const {
+        Mid m;
+        if constexpr (K == 1) {
+            float b, c;
+            if constexpr (sizeof(T) == 4)
+                b = __uint_as_float(in.w[0]), c = __uint_as_float(in.w[1]);
+            else
+                ki::unpair(b, c, widen2<T>(in.w[0]));
+            m.a[0] = ki::pair(ki::exp2_fast(in.x.x * A[0]), 0.0f);
+            m.add[0] = ki::pair(in.x.y * b, 0.0f);
+            m.c[0] = ki::pair(c, 0.0f);
+        } else {
+            const ki::f32x2 s = ki::pair(in.x.x), su = ki::pair(in.x.y);
+#pragma unroll
+            for (int k = 0; k < K; k += 2) {
+                ki::f32x2 b;
+                if constexpr (sizeof(T) == 4) {
+                    b = ki::pair(__uint_as_float(in.w[k]), __uint_as_float(in.w[k + 1]));
+                    m.c[k / 2] = ki::pair(__uint_as_float(in.w[K + k]), __uint_as_float(in.w[K + k + 1]));
+                } else {
+                    b = widen2<T>(in.w[k / 2]);
+                    m.c[k / 2] = widen2<T>(in.w[(K + k) / 2]);
+                }
+                float e0, e1;
+                ki::unpair(e0, e1, ki::mul2(s, ki::pair(A[k], A[k + 1])));
+                m.a[k / 2] = ki::pair(ki::exp2_fast(e0), ki::exp2_fast(e1));
+                m.add[k / 2] = ki::mul2(su, b);
+            }
+        }
+        return m;
+    }
+    __device__ __forceinline__ float apply(const Mid& m) {
+        float lo, hi;
+        if constexpr (K == 1) {
+            float a, add, c;
+            ki::unpair(a, hi, m.a[0]);
+            ki::unpair(add, hi, m.add[0]);
+            ki::unpair(c, hi, m.c[0]);
+            h[0] = fmaf(a, h[0], add);
+            return c * h[0];
+        } else {
+            ki::f32x2 sum = 0;
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const ki::f32x2 hh = ki::fma2(m.a[k], ki::pair(h[2 * k], h[2 * k + 1]), m.add[k]);
+                ki::unpair(h[2 * k], h[2 * k + 1], hh);
+                sum = k == 0 ? ki::mul2(m.c[k], hh) : ki::fma2(m.c[k], hh, sum);
+            }
+            ki::unpair(lo, hi, sum);
+            return lo + hi;
+        }
+    }
+    // Tokens 0 to tn of a chunk.  The arrays do not overlap: loads of later tokens pass the stores of earlier ones.
+    // Loads ahead wrap around at the chunk's end; what they bring is not used.
+    __device__ __forceinline__ void chunk(const float2* __restrict__ step, const uint32_t* __restrict__ bc,
+                                          float* __restrict__ part, int tn, int tid) {
+        auto at = [&](int t) { return L::part_at(t, tid >> 2) * 4 + (tid & 3); };
+        if (tn >= kTime) {
+            Mid m = decays(load(step, bc, 0));
+            In in = load(step, bc, 1);
+#pragma unroll 1
+            for (int t0 = 0; t0 < kTime; t0 += kUnroll) {
+#pragma unroll
+                for (int t = 0; t < kUnroll; ++t) {
+                    const In in2 = load(step, bc, t + 2 < kUnroll ? t0 + t + 2 : (t0 + t + 2) & (kTime - 1));
+                    const Mid m2 = decays(in);
+                    part[at(t0 + t)] = apply(m);
+                    m = m2;
+                    in = in2;
+                }
+            }
+        } else {
+            for (int t = 0; t < tn; ++t) part[at(t)] = apply(decays(load(step, bc, t)));
+        }
+    }
+};
+
+template <class T, int LPC, int K>
+__global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ? 2 : 1)
+    scan_kernel(const ScanArgs a, int tiles) {
+    using L = Tile<T, LPC, K>;
+    constexpr int DT = L::DT, VC = L::VC, NB = L::NB;
+    extern __shared__ __align__(16) uint8_t smem[];
+    typename L::Stage* stage = reinterpret_cast<typename L::Stage*>(smem);
     const ki::Sequences& q = a.seq;
-    if (blockIdx.x == 0) q.check(threadIdx.x, kThreads);
+    if (blockIdx.x == 0) q.check(threadIdx.x, kLanes + kHelpers);
     const int seq = blockIdx.x / (tiles * a.groups);
     const int rest = blockIdx.x % (tiles * a.groups);
     const int g = rest / tiles;
@@ -73,83 +273,171 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(const ScanArgs a, int ti
     const int in0 = (rest % tiles) * DT;  // first channel within the group
     const int width = min(DT, per - in0);
     const int d0 = g * per + in0;
-    const int b = q.begin(seq), e = max(b, q.begin(seq + 1));
+    const int b0 = q.begin(seq), len = max(0, q.begin(seq + 1) - b0);
     float* st = nullptr;
     if (a.state) {
         const int64_t slot = q.slot(seq);
         if (slot < 0) return;  // padding: its rows and state stay as they are
         st = a.state + (size_t)slot * a.state_ld;
     }
-    const int lane = threadIdx.x % LPC, dl = threadIdx.x / LPC;
-    const int n0 = lane * K;
-    const bool live = dl < width;
-    float A[K], h[K];
+    const int chunks = (len + kTime - 1) / kTime;
+
+    if (threadIdx.x < kLanes) {
+        const int dl = threadIdx.x / LPC, ln = threadIdx.x % LPC;
+        const bool keep = st && q.continues(seq);
+        Lane<T, LPC, K> lane;
+        lane.A[2 * lane.P - 1] = lane.h[2 * lane.P - 1] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const bool on = live && n0 + k < a.states;
-        const size_t at = (size_t)(d0 + dl) * a.states + n0 + k;
-        A[k] = on ? a.A[at] * ki::kLog2e : 0.0f;
-        h[k] = on && st && q.continues(seq) ? st[at] : 0.0f;
-    }
-    const T* u = static_cast<const T*>(a.u);
-    const T* delta = static_cast<const T*>(a.delta);
-    const T* B = static_cast<const T*>(a.B) + (size_t)g * a.states;
-    const T* C = static_cast<const T*>(a.C) + (size_t)g * a.states;
-    for (int t0 = b; t0 < e; t0 += TC) {
-        const int tn = min(TC, e - t0);
-        for (int i = threadIdx.x; i < tn * DT; i += kThreads) {
-            const int t = i / DT, d = i % DT;
-            float2 v = make_float2(0.0f, 0.0f);
-            if (d < width) {
-                float s = ki::to_f32(delta[(size_t)(t0 + t) * a.ldd + d0 + d]);
-                if (a.delta_bias) s += a.delta_bias[d0 + d];
-                if (a.soft) s = ki::softplus(s);
-                v = make_float2(s, s * ki::to_f32(u[(size_t)(t0 + t) * a.ldu + d0 + d]));
-            }
-            s_step[t][d] = v;
-        }
-        for (int i = threadIdx.x; i < tn * NP; i += kThreads) {
-            const int t = i / NP, n = i % NP;
-            float2 v = make_float2(0.0f, 0.0f);
-            if (n < a.states)
-                v = make_float2(ki::to_f32(B[(size_t)(t0 + t) * a.ldb + n]), ki::to_f32(C[(size_t)(t0 + t) * a.ldc + n]));
-            s_bc[t][n] = v;
+        for (int k = 0; k < K; ++k) {
+            const bool on = dl < width && ln * K + k < a.states;
+            const size_t at = (size_t)(d0 + dl) * a.states + ln * K + k;
+            lane.A[k] = on ? a.A[at] * ki::kLog2e : 0.0f;
+            lane.h[k] = on && keep ? st[at] : 0.0f;
         }
         __syncthreads();
-        for (int t = 0; t < tn; t += LPC) {
-            float p[LPC];
+        for (int i = 0; i < chunks; ++i) {
+            typename L::Stage& s = stage[i & 1];
+            lane.chunk(s.step + dl, s.bc + ln * L::GW, reinterpret_cast<float*>(s.part), len - i * kTime, threadIdx.x);
+            __syncthreads();
+        }
+        if (st) {
 #pragma unroll
-            for (int i = 0; i < LPC; ++i) {
-                p[i] = 0.0f;
-                if (t + i < tn) {
-                    const float2 x = s_step[t + i][dl];
+            for (int k = 0; k < K; ++k)
+                if (dl < width && ln * K + k < a.states) st[(size_t)(d0 + dl) * a.states + ln * K + k] = lane.h[k];
+        }
+        return;
+    }
+
+    // Helper threads: VC channels, and a share of B and C, of one token of each chunk.
+    const int tid = threadIdx.x - kLanes, t = tid / kShare, sh = tid % kShare;
+    const int c0 = sh * VC, n = min(max(width - c0, 0), VC);
+    const T* u = static_cast<const T*>(a.u) + d0 + c0;
+    const T* delta = static_cast<const T*>(a.delta) + d0 + c0;
+    const T* z = a.z ? static_cast<const T*>(a.z) + d0 + c0 : nullptr;
+    T* y = static_cast<T*>(a.y) + d0 + c0;
+    const T* B = static_cast<const T*>(a.B) + (size_t)g * a.states + sh * NB;
+    const T* C = static_cast<const T*>(a.C) + (size_t)g * a.states + sh * NB;
+    const int states = min(max(a.states - sh * NB, 0), NB);
+    float bias[VC], skip[VC];
 #pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        const float2 bc = s_bc[t + i][n0 + k];
-                        h[k] = fmaf(ki::exp2_fast(x.x * A[k]), h[k], x.y * bc.x);
-                        p[i] = fmaf(bc.y, h[k], p[i]);
-                    }
+    for (int j = 0; j < VC; ++j) {
+        bias[j] = a.delta_bias && j < n ? a.delta_bias[d0 + c0 + j] : 0.0f;
+        skip[j] = a.D && j < n ? a.D[d0 + c0 + j] : 0.0f;
+    }
+    constexpr bool kAhead = NB <= 8;  // few enough states to be loaded a chunk ahead
+    constexpr int NC = kAhead ? NB : K;
+    struct Loads {
+        Raw<T, VC> delta, u;
+        Raw<T, NC> b, c;
+    } next = {}, now = {};         // the chunk after the next one (in flight), the next one
+    Raw<T, VC> u1 = {}, u0, znext = {}, z0;  // u of the chunk being computed and of the one before it; z of those
+
+    auto load = [&](int i) {
+        const int at = i * kTime + t;
+        if (at >= len) return;
+        const size_t row = (size_t)b0 + at;
+        next.delta.load(delta + row * a.ldd, a.vec, n);
+        next.u.load(u + row * a.ldu, a.vec, n);
+        if constexpr (kAhead) {
+            next.b.load(B + row * a.ldb, a.vec_b, states);
+            next.c.load(C + row * a.ldc, a.vec_c, states);
+        }
+        if (n > 0 && at + 2 * kTime < len) {  // DRAM's part of the latency is taken two chunks earlier still
+            const size_t far = row + 2 * kTime;
+            prefetch(delta + far * a.ldd);
+            prefetch(u + far * a.ldu);
+            if (z) prefetch(z + far * a.ldz);
+        }
+    };
+    auto load_z = [&](int i) {
+        if (z && i * kTime + t < len) znext.load(z + ((size_t)b0 + (size_t)i * kTime + t) * a.ldz, a.vec, n);
+    };
+    auto take = [&]() {
+        u0 = u1;
+        u1 = now.u;
+        now = next;
+        z0 = znext;
+    };
+    auto fill = [&](int i) {  // the loaded chunk, as the compute threads want it
+        if (i * kTime + t >= len) return;
+        typename L::Stage& s = stage[i & 1];
+        float2* step = s.step + t * L::ROW + c0;
+#pragma unroll
+        for (int j = 0; j < VC; j += 2) {
+            constexpr int one = VC > 1 ? 1 : 0;
+            ki::f32x2 x = ki::add2(ki::pair(ki::to_f32(now.delta.get(j)), ki::to_f32(now.delta.get(j + one))),
+                                   ki::pair(bias[j], bias[j + one]));
+            if (a.soft) x = ki::softplus2(x);
+            float x0, x1, v0, v1;
+            ki::unpair(x0, x1, x);
+            ki::unpair(v0, v1, ki::mul2(x, ki::pair(ki::to_f32(now.u.get(j)), ki::to_f32(now.u.get(j + one)))));
+            step[j] = make_float2(x0, v0);
+            if (one) step[j + one] = make_float2(x1, v1);
+        }
+        const size_t row = (size_t)b0 + (size_t)i * kTime + t;
+#pragma unroll
+        for (int j = 0; j < NB; j += K) {  // a compute lane's states
+            if constexpr (!kAhead) {
+                now.b.load(B + row * a.ldb + j, a.vec_b, states - j);
+                now.c.load(C + row * a.ldc + j, a.vec_c, states - j);
+            }
+            const int at = kAhead ? j : 0;
+            uint32_t w[L::GW];
+            if constexpr (K * sizeof(T) >= 4) {
+#pragma unroll
+                for (int k = 0; k < L::GW / 2; ++k) {
+                    w[k] = now.b.w[at * (int)sizeof(T) / 4 + k];
+                    w[L::GW / 2 + k] = now.c.w[at * (int)sizeof(T) / 4 + k];
                 }
+            } else {
+                w[0] = now.b.half(at) | now.c.half(at) << 16;
             }
-            const float sum = fold_lanes<LPC>(p, lane);
-            if (t + lane < tn) s_y[t + lane][dl] = sum;
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < tn * DT; i += kThreads) {
-            const int t = i / DT, d = i % DT;
-            if (d < width) {
-                float y = s_y[t][d];
-                if (a.D) y = fmaf(a.D[d0 + d], ki::to_f32(u[(size_t)(t0 + t) * a.ldu + d0 + d]), y);
-                if (a.z) y *= ki::silu(ki::to_f32(static_cast<const T*>(a.z)[(size_t)(t0 + t) * a.ldz + d0 + d]));
-                static_cast<T*>(a.y)[(size_t)(t0 + t) * a.ldy + d0 + d] = ki::from_f32<T>(y);
-            }
-        }
-    }
-    if (st && live) {
+            constexpr int W = L::GW < 4 ? L::GW : 4;
+            uint32_t* to = s.bc + (t * LPC + (sh * NB + j) / K) * L::GW;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (n0 + k < a.states) st[(size_t)(d0 + dl) * a.states + n0 + k] = h[k];
+            for (int k = 0; k < L::GW; k += W) {
+                ki::Vec<uint32_t, W> v;
+#pragma unroll
+                for (int e = 0; e < W; ++e) v.e[e] = w[k + e];
+                ki::store_vec(to + k, v);
+            }
+        }
+    };
+    auto finish = [&](int i) {  // outputs of a computed chunk
+        if (i * kTime + t >= len || n == 0) return;
+        const size_t row = (size_t)b0 + (size_t)i * kTime + t;
+        typename L::Stage& s = stage[i & 1];
+        Raw<T, VC> out = {};
+#pragma unroll
+        for (int j = 0; j < VC; ++j) {
+            float v = 0.0f;
+#pragma unroll
+            for (int k = 0; k < LPC / 4; ++k) {
+                const float4 p = s.part[L::part_at(t, (c0 + j) * (LPC / 4) + k)];
+                v += (p.x + p.y) + (p.z + p.w);
+            }
+            if (a.D) v = fmaf(skip[j], ki::to_f32(u0.get(j)), v);
+            if (z) v *= ki::silu(ki::to_f32(z0.get(j)));
+            out.set(j, ki::from_f32<T>(v));
+        }
+        out.store(y + row * a.ldy, a.vec, n);
+    };
+
+    load(0);
+    take();
+    load(1);
+    fill(0);
+    __syncthreads();
+    for (int i = 0; i < chunks; ++i) {
+        take();
+        load(i + 2);
+        load_z(i);
+        if (i > 0) finish(i - 1);
+        fill(i + 1);
+        __syncthreads();
     }
+    take();
+    if (chunks > 0) finish(chunks - 1);
 }
 
 // One token per row: row r continues slot slots[r].  LPC lanes share a channel.
@@ -190,26 +478,48 @@ __global__ void __launch_bounds__(kThreads) scan_step_kernel(const ScanArgs a, i
 }
 
 template <class T, int LPC, int K>
-int launch(ki_ctx* ctx, const ScanArgs& a, cudaStream_t s) {
-    constexpr int DT = kThreads / LPC;
-    const long long tiles = (a.channels / a.groups + DT - 1) / DT;
+int launch(ki_ctx* ctx, ScanArgs& a, cudaStream_t s) {
+    using L = Tile<T, LPC, K>;
+    const int per = a.channels / a.groups;
+    const long long tiles = (per + L::DT - 1) / L::DT;
     const long long blocks = tiles * a.groups * a.seq.count;
     if (blocks > 0x7fffffffll) return ki::set_error(ctx, KI_ERR_ARG, "selective_scan: too many sequences");
-    scan_kernel<T, LPC, K><<<(unsigned)blocks, kThreads, 0, s>>>(a, (int)tiles);
+    const size_t es = sizeof(T), w = L::VC * es > 16 ? 16 : L::VC * es;
+    const bool one = a.seq.tokens <= 1;
+    a.vec = ki::rows_aligned(a.u, one ? 0 : a.ldu, es, w) && ki::rows_aligned(a.delta, one ? 0 : a.ldd, es, w) &&
+            ki::rows_aligned(a.z, one || !a.z ? 0 : a.ldz, es, w) && ki::rows_aligned(a.y, one ? 0 : a.ldy, es, w) &&
+            (a.groups == 1 || per * es % w == 0);
+    const size_t wb = (L::NB <= 8 ? L::NB : K) * es, wv = wb > 16 ? 16 : wb;
+    const bool whole = a.groups == 1 || a.states * es % wv == 0;
+    a.vec_b = whole && ki::rows_aligned(a.B, one ? 0 : a.ldb, es, wv);
+    a.vec_c = whole && ki::rows_aligned(a.C, one ? 0 : a.ldc, es, wv);
+    constexpr int smem = 2 * sizeof(typename L::Stage);
+    auto kern = scan_kernel<T, LPC, K>;
+    KI_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kern<<<(unsigned)blocks, kLanes + kHelpers, smem, s>>>(a, (int)tiles);
     return ki::check_launch(ctx, "selective_scan launch");
 }
 
 template <class T>
-int launch_scan(ki_ctx* ctx, const ScanArgs& a, cudaStream_t s) {
-    if (a.states <= 16) return launch<T, 16, 1>(ctx, a, s);
-    if (a.states <= 32) return launch<T, 16, 2>(ctx, a, s);
+int launch_scan(ki_ctx* ctx, ScanArgs& a, cudaStream_t s) {
+    // Blocks if every lane held four states.  A lane with fewer takes less time for a token (D = 256, 2048 tokens, N = 16:
+    // 77 us with four states, 54 with two, 43 with one), but more of the SM's issue slots in all, so fewer states pay
+    // while every block has an SM of its own (D = 4096: 79, 85, 128 us).
+    const int per = a.channels / a.groups, sms = ctx->sm_count;
+    auto blocks = [&](int channels) { return (long long)a.seq.count * a.groups * ((per + channels - 1) / channels); };
+    if (a.states <= 8) return blocks(16) <= sms ? launch<T, 8, 1>(ctx, a, s) : launch<T, 4, 2>(ctx, a, s);
+    if (a.states <= 16) {
+        if (blocks(8) <= sms) return launch<T, 16, 1>(ctx, a, s);
+        return blocks(16) <= sms ? launch<T, 8, 2>(ctx, a, s) : launch<T, 4, 4>(ctx, a, s);
+    }
+    if (a.states <= 32) return blocks(8) <= sms ? launch<T, 16, 2>(ctx, a, s) : launch<T, 8, 4>(ctx, a, s);
     if (a.states <= 64) return launch<T, 16, 4>(ctx, a, s);
     if (a.states <= 128) return launch<T, 16, 8>(ctx, a, s);
-    return launch<T, 16, 16>(ctx, a, s);
+    return launch<T, 32, 8>(ctx, a, s);
 }
 
 template <class T>
-int launch_step(ki_ctx* ctx, const ScanArgs& a, cudaStream_t s) {
+int launch_step(ki_ctx* ctx, ScanArgs& a, cudaStream_t s) {
     constexpr int LPC = 8, DT = kThreads / LPC;
     const long long tiles = (a.channels + DT - 1) / DT;
     if (tiles * a.seq.count > 0x7fffffffll) return ki::set_error(ctx, KI_ERR_ARG, "selective_scan_step: too many rows");
@@ -283,7 +593,7 @@ extern "C" int ki_selective_scan(ki_ctx* ctx, int dtype, const void* d_u, size_t
         return ki::set_error(ctx, KI_ERR_ARG, "selective_scan: too many sequences or slots");
     if (!d_offsets && seqs != 1) return ki::set_error(ctx, KI_ERR_ARG, "selective_scan: several sequences need offsets");
     ScanArgs a{d_u, ldu, d_delta, ldd, d_A, d_B, ldb, d_C, ldc, d_D, d_z, ldz, d_delta_bias, d_state, state_ld, d_y, ldy,
-               0, 0, 0, softplus != 0, {d_offsets, d_slots, d_initial, (int)seqs, 0, (int64_t)slots, nullptr}};
+               0, 0, 0, softplus != 0, false, false, false, {d_offsets, d_slots, d_initial, (int)seqs, 0, (int64_t)slots, nullptr}};
     return scan(ctx, "selective_scan", dtype, a, tokens, channels, states, groups, false, stream);
 }
 
@@ -298,6 +608,6 @@ extern "C" int ki_selective_scan_step(ki_ctx* ctx, int dtype, const void* d_u, s
         return ki::set_error(ctx, KI_ERR_ARG, "selective_scan_step: too many rows or slots");
     if (!d_state) return ki::set_error(ctx, KI_ERR_ARG, "selective_scan_step: null pointer");
     ScanArgs a{d_u, ldu, d_delta, ldd, d_A, d_B, ldb, d_C, ldc, d_D, d_z, ldz, d_delta_bias, d_state, state_ld, d_y, ldy,
-               0, 0, 0, softplus != 0, {nullptr, d_slots, nullptr, (int)rows, 0, (int64_t)slots, nullptr}};
+               0, 0, 0, softplus != 0, false, false, false, {nullptr, d_slots, nullptr, (int)rows, 0, (int64_t)slots, nullptr}};
     return scan(ctx, "selective_scan_step", dtype, a, rows, channels, states, groups, true, stream);
 }
