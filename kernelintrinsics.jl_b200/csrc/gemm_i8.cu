@@ -7,16 +7,21 @@
 // channels in Float32, Float16 or BFloat16.  The Int32 sums are exact (inner <= 131071, where 128 * 128
 // * inner still fits), so the result does not depend on the order of the sums or on how they are split.
 //
-// The weights are the MMA's M side: a CTA holds 128 channels x BN tokens, lanes of TMEM are channels and
-// columns are tokens.  A warp's store of one column is then 32 neighbouring channels of one token, and a
-// few tokens (BN = 16) cost a few columns instead of a mostly empty tile of 128 rows.
-//   warp 0     loads K blocks of 128 into a ring of stages (TMA, 128-byte swizzle); rows that are not
-//              16-byte aligned are loaded by warps 2-5 with plain loads instead (load_rows);
+// The weights are the MMA's M side: lanes of TMEM are channels and columns are tokens.  A warp's store of one column
+// is then 32 neighbouring channels of one token, whatever the sizes and strides of C, and a few tokens cost a few
+// columns instead of a mostly empty tile of 128 rows.  Two kernels:
+//
+// gemm_i8_kernel, one tile of 128 channels x BN tokens per CTA:
+//   warp 0     loads K blocks of 128 into a ring of stages (TMA, 128-byte swizzle);
 //   warp 1     allocates TMEM and issues the MMAs (M 128, N BN, K 32) from one thread;
-//   warps 2-5  epilogue: TMEM -> registers -> scales -> C.
+//   warps 2-5  (2-9 from BN = 64) epilogue: TMEM -> registers -> scales -> C.
 // With few tiles the K blocks of a tile are split over the CTAs of a cluster; each CTA then leaves its
 // Int32 sums in its own shared memory and adds up and stores a share of the tile's columns, read from
-// every CTA of the cluster.
+// every CTA of the cluster.  Rows that are not 16-byte aligned are loaded by warps 2-9 with plain loads.
+//
+// gemm_i8_pair_kernel, persistent CTA pairs on tiles of 256 channels x 256 tokens (cta_group::2): each CTA loads
+// 128 rows of either operand, each SM's TMEM holds two accumulators of its 128 channels x 256 tokens, so that the
+// epilogue of a tile runs beside the next tile's MMAs.
 //
 // Every mbarrier wait is bounded, as in gemm_e4m3.cu.
 #include "ki/layer.cuh"
@@ -25,8 +30,12 @@
 
 namespace {
 
+#ifndef KI_I8_PAIRS
+#define KI_I8_PAIRS 60
+#endif
 constexpr int BM = 128, BK = 128;
-constexpr int THREADS = 192;
+constexpr int LOADERS = 16;  // warps that load rows which TMA cannot, 16 each
+constexpr int THREADS_ROWS = 64 + 32 * LOADERS;
 constexpr int W_BYTES = BM * BK;
 constexpr int MAX_SPLIT = 8;
 
@@ -35,15 +44,20 @@ constexpr uint32_t idesc(int bn) {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 }
 
-template <int BN>
+template <int BN, bool TMA>
 struct Shape {
     static constexpr int X_BYTES = BN * BK;
     static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
-    static constexpr int STAGES = BN <= 64 ? 5 : 4;
+    // two CTAs per SM, but one with a deeper ring for the widest tiles
+    static constexpr int STAGES = BN <= 16 ? 6 : BN <= 32 ? 5 : BN <= 64 ? 4 : 6;
     static constexpr int SUM_BYTES = BM * BN * 4;  // a split's Int32 sums, over the ring
     static constexpr int RING_BYTES = STAGES * STAGE_BYTES > SUM_BYTES ? STAGES * STAGE_BYTES : SUM_BYTES;
-    static constexpr int SMEM_BYTES = 1024 + RING_BYTES + 256;
+    static constexpr int SA_COLS = BN < 32 ? 32 : BN;  // the tokens' scales, behind the barriers
+    static constexpr int SMEM_BYTES = 1024 + RING_BYTES + 256 + 4 * SA_COLS;
     static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
+    static constexpr int EPI_WARPS = BN < 64 ? 4 : 8;  // four per 32 TMEM lanes, or eight with half of the columns each
+    static constexpr int EPI_COLS = BN < 64 ? TMEM_COLS : BN / 2;
+    static constexpr int THREADS = 64 + 32 * EPI_WARPS;
 };
 
 struct GemmArgs {
@@ -71,50 +85,96 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t wdesc, uint64_t
         : "memory");
 }
 
-// 16 bytes from p, of which the first nb (0 to 16) exist and the others read as zero; any alignment.
-// Only 4-byte words that hold one of those bytes are read.
-__device__ __forceinline__ uint4 load16(const int8_t* p, int nb) {
-    uint32_t w[5];
-    const uintptr_t at = (uintptr_t)p;
-    const uint32_t off = (uint32_t)(at & 3);
-    const uint32_t* q = reinterpret_cast<const uint32_t*>(at - off);
+// 16 rows of a matrix, a K block at a time, loaded by one warp from rows that start at any byte.  Lane l takes the
+// 4-byte word l of every row, and lane r word 32 of row r; a byte shift by the row's misalignment (between neighbouring
+// lanes' words) gives the row's bytes.  Rows r, r + 4, ... share their misalignment.  Only words that hold a byte of a
+// row are read, and what lies behind the rows' end or the last row is zero.  Whole blocks of existing rows, nearly
+// all, take a path without those tests.
+struct Rows {
+    static constexpr int N = 16;
+    const int8_t* x;  // the first row
+    size_t ld;
+    int rows;         // that exist
+    int k;
+    int lane;
+    uint32_t off[4];  // misalignment of rows 0 to 3
+    struct Words {
+        uint32_t w[N], last;
+    };
+    __device__ __forceinline__ Rows(const int8_t* base, size_t ld_, int row0, int end, int k_, int lane_)
+        : x(base + (size_t)row0 * ld_), ld(ld_), rows(min(end - row0, N)), k(k_), lane(lane_) {
 #pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = nb > 0 && 4 * i < (int)off + nb ? __ldg(q + i) : 0u;
-    uint32_t o[4];
+        for (int j = 0; j < 4; ++j) off[j] = (uint32_t)((uintptr_t)x + j * ld) & 3;  // the same in every K block
+    }
+    __device__ __forceinline__ void load(Words& v, int k0) const {
+        const int8_t* p = x + k0;
+        const int bytes = min(k - k0, BK);
+        if (rows == N && bytes == BK) {
+            const int8_t* q[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        o[i] = __funnelshift_r(w[i], w[i + 1], 8 * off);
-        const int v = min(max(nb - 4 * i, 0), 4);
-        o[i] &= v == 4 ? 0xffffffffu : (1u << (8 * v)) - 1u;
+            for (int j = 0; j < 4; ++j) q[j] = p + j * ld - off[j] + 4 * lane;
+#pragma unroll
+            for (int r = 0; r < N; ++r) {
+                v.w[r] = __ldg(reinterpret_cast<const uint32_t*>(q[r & 3]));
+                q[r & 3] += 4 * ld;
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < N; ++r)
+                v.w[r] = r < rows && 4 * lane < (int)off[r & 3] + bytes
+                             ? __ldg(reinterpret_cast<const uint32_t*>(p + r * ld - off[r & 3]) + lane)
+                             : 0u;
+        }
+        const uint32_t o = (uint32_t)((uintptr_t)x + lane * ld) & 3;
+        v.last = lane < rows && BK < (int)o + bytes ? __ldg(reinterpret_cast<const uint32_t*>(p + lane * ld - o) + 32) : 0u;
     }
-    return make_uint4(o[0], o[1], o[2], o[3]);
-}
-
-// `count` rows of a K block to shared memory in the layout that the 128-byte swizzle gives a TMA tile:
-// row r at 128 r, its 16-byte pieces exchanged by r mod 8.  Run by 128 threads.
-__device__ __forceinline__ void load_rows(uint32_t dst, const int8_t* x, size_t ld, int row0, int rows, int k0, int k,
-                                          int count, int tid) {
-    for (int i = tid; i < count * 8; i += 128) {
-        const int r = i >> 3, j = i & 7;
-        const int kk = k0 + 16 * j;
-        const int nb = row0 + r < rows ? min(max(k - kk, 0), 16) : 0;
-        const uint4 v = load16(x + (nb > 0 ? (size_t)(row0 + r) * ld + kk : 0), nb);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)(r * 128 + ((j ^ (r & 7)) << 4))),
-                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                     : "memory");
+    // To shared memory at dst, as a TMA tile with the 128-byte swizzle: row r at 128 r, its 16-byte pieces exchanged by r mod 8.
+    __device__ __forceinline__ void store(const Words& v, uint32_t dst, int k0) const {
+        const int left = min(max(k - k0 - 4 * lane, 0), 4);  // bytes of this lane's word
+        const uint32_t mask = left == 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            const uint32_t end = __shfl_sync(0xffffffffu, v.last, r);
+            uint32_t next = __shfl_down_sync(0xffffffffu, v.w[r], 1);
+            if (lane == 31) next = end;
+            const uint32_t b = __funnelshift_r(v.w[r], next, 8 * off[r & 3]) & mask;
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + (uint32_t)(r * 128 + ((4 * lane) ^ ((r & 7) << 4)))), "r"(b)
+                         : "memory");
+        }
     }
-}
+};
 
 template <class O>
 __device__ __forceinline__ O scaled(int32_t v, float sa, float sw, float bias) {
     return ki::from_f32<O>(fmaf((float)v * sa, sw, bias));
 }
 
+// 32 tokens' sums of a channel: scaled and stored to column c of their rows, as many as there are.
+template <class O>
+__device__ __forceinline__ void store_columns(O* c, size_t ldc, const uint32_t (&v)[32], const float* sa, float sw,
+                                              float bias, int count) {
+    if (count >= 32) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(sa + j);
+            c[0] = scaled<O>((int)v[j], s.x, sw, bias);
+            c[ldc] = scaled<O>((int)v[j + 1], s.y, sw, bias);
+            c[2 * ldc] = scaled<O>((int)v[j + 2], s.z, sw, bias);
+            c[3 * ldc] = scaled<O>((int)v[j + 3], s.w, sw, bias);
+            c += 4 * ldc;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < count) c[(size_t)j * ldc] = scaled<O>((int)v[j], sa[j], sw, bias);
+    }
+}
+
 template <int BN, class O, bool TMA>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(TMA ? Shape<BN, TMA>::THREADS : THREADS_ROWS, 1)
     gemm_i8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const GemmArgs g,
                    int split) {
-    using S = Shape<BN>;
+    using S = Shape<BN, TMA>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = ki::smem_addr(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -123,6 +183,7 @@ __global__ void __launch_bounds__(THREADS)
     uint8_t* gbase = smem_raw + (base - raw);
     volatile int* abort = reinterpret_cast<volatile int*>(gbase + S::RING_BYTES + 128);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(gbase + S::RING_BYTES + 136);
+    float* scales = reinterpret_cast<float*>(gbase + S::RING_BYTES + 256);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int part = blockIdx.x % split, tile = blockIdx.x / split;
@@ -130,9 +191,10 @@ __global__ void __launch_bounds__(THREADS)
     const int blocks = (g.k + BK - 1) / BK;
     const int kb0 = (int)((long long)blocks * part / split), kb1 = (int)((long long)blocks * (part + 1) / split);
 
+    for (int i = threadIdx.x; i < S::SA_COLS; i += blockDim.x) scales[i] = i < BN && m0 + i < g.m ? g.sa[m0 + i] : 0.0f;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full0 + 8 * s), "r"(TMA ? 1 : 128));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full0 + 8 * s), "r"(TMA ? 1 : LOADERS));
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty0 + 8 * s));
         }
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(tfull));
@@ -199,41 +261,53 @@ __global__ void __launch_bounds__(THREADS)
             wait_drain(tfull, 0, g.status, g.timeout_ns);
         }
     } else if (!TMA && warp >= 2) {
-        const int tid = threadIdx.x - 64;
+        // W's 128 rows, then A's BN, 16 to a warp; a block's loads are in flight while the one before it is stored
+        static_assert(BM + BN <= Rows::N * LOADERS && BN % Rows::N == 0, "16 rows per warp");
+        const int r0 = Rows::N * (warp - 2);
+        const bool some = r0 < BM + BN, isw = r0 < BM;
+        const Rows rows(isw ? g.w : g.a, isw ? g.ldw : g.lda, isw ? n0 + r0 : m0 + r0 - BM, isw ? g.n : min(g.m, m0 + BN),
+                        g.k, lane);
         int s = 0;
         uint32_t ph = 1;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        auto put = [&](const Rows::Words& v, int kb) {
             int ok = 0;
             if (lane == 0) ok = wait_bar(empty0 + 8 * s, ph, abort, g.status, g.timeout_ns) ? 1 : 0;
-            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-            const uint32_t sw = ring + s * S::STAGE_BYTES;
-            load_rows(sw, g.w, g.ldw, n0, g.n, kb * BK, g.k, BM, tid);
-            load_rows(sw + W_BYTES, g.a, g.lda, m0, g.m, kb * BK, g.k, BN, tid);
+            if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
+            if (some) rows.store(v, ring + s * S::STAGE_BYTES + r0 * BK, kb * BK);
             ki::fence_proxy_async_smem();
-            mbar_arrive(full0 + 8 * s);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full0 + 8 * s);
             if (++s == S::STAGES) {
                 s = 0;
                 ph ^= 1;
             }
+            return true;
+        };
+        Rows::Words even, odd;
+        if (some && kb0 < kb1) rows.load(even, kb0 * BK);
+        for (int kb = kb0; kb < kb1; kb += 2) {
+            if (some && kb + 1 < kb1) rows.load(odd, (kb + 1) * BK);
+            if (!put(even, kb) || kb + 1 == kb1) break;
+            if (some && kb + 2 < kb1) rows.load(even, (kb + 2) * BK);
+            if (!put(odd, kb + 1)) break;
         }
     }
     __syncwarp();
 
-    if (warp >= 2) {
+    if (warp >= 2 && warp < 2 + S::EPI_WARPS) {
         int ok = 0;
         if (lane == 0) ok = wait_bar(tfull, 0, abort, g.status, g.timeout_ns) ? 1 : 0;
         ok = __shfl_sync(0xffffffffu, ok, 0);
         tc_fence_after();
-        const int row = (warp & 3) * 32;  // TMEM lanes that this warp may read
+        const int row = (warp & 3) * 32;                              // TMEM lanes that this warp may read
+        const int first = (warp - 2) / 4 * S::EPI_COLS;               // and its columns
         const int n = n0 + row + lane;
         const bool on = n < g.n;
         const float sw = on ? g.sw[n] : 0.0f, bias = on && g.bias ? g.bias[n] : 0.0f;
-        O* c = static_cast<O*>(g.c) + n;
-        constexpr int STEP = BN < 32 ? BN : 32;
         if (ok) {
 #pragma unroll 1
-            for (int c0 = 0; c0 < BN; c0 += STEP) {
-                if (split == 1 && m0 + c0 >= g.m) break;
+            for (int c0 = first; c0 < first + S::EPI_COLS; c0 += 32) {
+                if (m0 + c0 >= g.m) break;
                 uint32_t v[32];
                 if (kb1 > kb0) {
                     KI_TMEM_LD_X32(tmem + ((uint32_t)row << 16) + (uint32_t)c0, v);
@@ -243,15 +317,12 @@ __global__ void __launch_bounds__(THREADS)
                     for (int j = 0; j < 32; ++j) v[j] = 0;
                 }
                 if (split == 1) {
-                    const float mine = m0 + c0 + lane < g.m ? g.sa[m0 + c0 + lane] : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < STEP; ++j) {
-                        const float sa = __shfl_sync(0xffffffffu, mine, j);
-                        if (on && m0 + c0 + j < g.m) c[(size_t)(m0 + c0 + j) * g.ldc] = scaled<O>((int)v[j], sa, sw, bias);
-                    }
+                    if (on)
+                        store_columns(static_cast<O*>(g.c) + (size_t)(m0 + c0) * g.ldc + n, g.ldc, v, scales + c0, sw, bias,
+                                      g.m - m0 - c0);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < STEP; ++j)
+                    for (int j = 0; j < (BN < 32 ? BN : 32); ++j)
                         asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + (uint32_t)(((c0 + j) * BM + row + lane) * 4)),
                                      "r"(v[j])
                                      : "memory");
@@ -262,23 +333,41 @@ __global__ void __launch_bounds__(THREADS)
     if (split > 1) {
         __syncwarp();
         cluster_sync_all();  // every part's sums are in its shared memory
-        if (warp >= 2 && !*abort) {
-            const int row = (warp & 3) * 32;
-            const int n = n0 + row + lane;
-            if (n < g.n) {
-                const float sw = g.sw[n], bias = g.bias ? g.bias[n] : 0.0f;
-                O* c = static_cast<O*>(g.c) + n;
-                for (int j = part; j < BN && m0 + j < g.m; j += split) {
-                    int32_t sum = 0;
-                    for (int p = 0; p < split; ++p) {
-                        int32_t v;
-                        asm volatile("ld.shared::cluster.b32 %0, [%1];"
-                                     : "=r"(v)
-                                     : "r"(map_rank(ring + (uint32_t)((j * BM + row + lane) * 4), (uint32_t)p))
-                                     : "memory");
-                        sum += v;
-                    }
-                    c[(size_t)(m0 + j) * g.ldc] = scaled<O>(sum, g.sa[m0 + j], sw, bias);
+        if (!*abort) {
+            // this CTA's share of the columns; a thread takes four neighbouring channels of one
+            const int n = n0 + 4 * lane, live = min(max(g.n - n, 0), 4);
+            const int columns = min(BN, g.m - m0);
+            float sw[4], bias[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sw[e] = e < live ? g.sw[n + e] : 0.0f;
+                bias[e] = e < live && g.bias ? g.bias[n + e] : 0.0f;
+            }
+            for (int j = part + split * warp; j < columns; j += split * (int)(blockDim.x / 32)) {
+                const uint32_t at = ring + (uint32_t)((j * BM + 4 * lane) * 4);
+                int4 v[MAX_SPLIT];
+#pragma unroll
+                for (int p = 0; p < MAX_SPLIT; ++p) {
+                    v[p] = make_int4(0, 0, 0, 0);
+                    if (p < split)
+                        asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(v[p].x), "=r"(v[p].y), "=r"(v[p].z), "=r"(v[p].w)
+                                     : "r"(map_rank(at, (uint32_t)p)));
+                }
+                int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int p = 0; p < MAX_SPLIT; ++p) sum[0] += v[p].x, sum[1] += v[p].y, sum[2] += v[p].z, sum[3] += v[p].w;
+                const float sa = scales[j];
+                O* c = static_cast<O*>(g.c) + (size_t)(m0 + j) * g.ldc + n;
+                ki::Vec<O, 4> o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o.e[e] = scaled<O>(sum[e], sa, sw[e], bias[e]);
+                if (live == 4 && (reinterpret_cast<uintptr_t>(c) % sizeof(o)) == 0) {
+                    ki::store_vec(c, o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < live) c[e] = o.e[e];
                 }
             }
         }
@@ -294,20 +383,273 @@ __global__ void __launch_bounds__(THREADS)
     }
 }
 
+// ---------------------------------------------------------------------------------------------
+// CTA pairs: rank r of a pair loads the channels [n0 + 128 r, +128) of W and the tokens [m0 + 128 r, +128) of A of each
+// K block (no multicast: every CTA loads only its own half); both CTAs' loads complete on rank 0's full barrier, and
+// rank 0's MMA thread issues M=256 N=256 K=32 MMAs that read both CTAs' shared memory at the same offsets.  The commits
+// arrive on the empty and accumulator-full barriers of both CTAs, both CTAs' epilogue warps on rank 0's
+// accumulator-empty barrier.
+// ---------------------------------------------------------------------------------------------
+constexpr int TILE2 = 256, STAGES2 = 6, ACCS2 = 2;
+constexpr int X2_BYTES = 128 * BK, STAGE2_BYTES = W_BYTES + X2_BYTES;
+constexpr int RING2_BYTES = STAGES2 * STAGE2_BYTES;
+constexpr int SA2_BYTES = ACCS2 * TILE2 * 4;  // the tokens' scales of the tile in either accumulator
+constexpr int SMEM2_BYTES = 1024 + RING2_BYTES + 256 + SA2_BYTES;
+constexpr uint32_t IDESC2 = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TILE2 >> 3) << 17) | ((uint32_t)(TILE2 >> 4) << 24);
+constexpr int EPI2_WARPS = 8;  // two per TMEM lane quadrant, half of the columns each
+constexpr int THREADS2 = 32 * (2 + EPI2_WARPS);
+
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t wdesc, uint64_t xdesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(wdesc), "l"(xdesc), "r"(IDESC2), "r"(accumulate)
+        : "memory");
+}
+
+// Output tile t -> (token block, channel block): groups of 16 token blocks are walked channel block by channel block,
+// so that the rows of A and W in flight stay in L2.
+__device__ __forceinline__ void tile2_coords(int t, int mtiles, int ntiles, int& mb, int& nb) {
+    const int group = t / (16 * ntiles), first = group * 16, size = min(16, mtiles - first);
+    const int in = t - group * 16 * ntiles;
+    mb = first + in % size;
+    nb = in / size;
+}
+
+template <class O>
+__global__ void __launch_bounds__(THREADS2, 1)
+    gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const GemmArgs g) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t raw = ki::smem_addr(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;  // identical in both CTAs: same kernel, same layout
+    const uint32_t ring = base, bars = base + RING2_BYTES;
+    const uint32_t full0 = bars, empty0 = bars + 8 * STAGES2, tfull0 = bars + 16 * STAGES2;
+    const uint32_t tempty0 = tfull0 + 8 * ACCS2, drain = tempty0 + 8 * ACCS2;
+    uint8_t* gbase = smem_raw + (base - raw);
+    volatile int* abort = reinterpret_cast<volatile int*>(gbase + RING2_BYTES + 192);
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(gbase + RING2_BYTES + 200);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const bool leader = rank == 0;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES2; ++s) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full0 + 8 * s));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty0 + 8 * s));
+        }
+        for (int b = 0; b < ACCS2; ++b) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(tfull0 + 8 * b));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tempty0 + 8 * b), "r"(2 * EPI2_WARPS));
+        }
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(drain));
+        *abort = 0;
+        ki::fence_mbar_init();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmW) : "memory");
+    }
+    if (warp == 1) {  // the same warp in both CTAs allocates the pair's TMEM together
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ki::smem_addr(tmem_holder)),
+                     "r"(ACCS2 * TILE2)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // both CTAs' barriers are initialised before any copy or arrive crosses over
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    const int tiles = g.mtiles * g.ntiles, blocks = (g.k + BK - 1) / BK;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint32_t full_lead0 = map_rank(full0, 0);
+            int s = 0;
+            uint32_t ph = 1;  // a fresh barrier's preceding phase counts as complete
+            uint32_t issued_ph[STAGES2];
+            bool issued[STAGES2];
+            for (int k = 0; k < STAGES2; ++k) issued[k] = false;
+            for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
+                int mb, nb;
+                tile2_coords(tile, g.mtiles, g.ntiles, mb, nb);
+                const int m0 = mb * TILE2 + 128 * (int)rank, n0 = nb * TILE2 + 128 * (int)rank;
+                for (int kb = 0; kb < blocks; ++kb) {
+                    if (!wait_bar(empty0 + 8 * s, ph, abort, g.status, g.timeout_ns)) break;
+                    const uint32_t sw = ring + s * STAGE2_BYTES;
+                    if (leader) mbar_expect_tx(full0 + 8 * s, 2 * STAGE2_BYTES);  // both CTAs' bytes
+                    tma_load_2d_pair(sw, &tmW, kb * BK, n0, full_lead0 + 8 * s);
+                    tma_load_2d_pair(sw + W_BYTES, &tmA, kb * BK, m0, full_lead0 + 8 * s);
+                    issued[s] = true;
+                    issued_ph[s] = ph ^ 1;  // the full-barrier phase this issue completes
+                    if (++s == STAGES2) {
+                        s = 0;
+                        ph ^= 1;
+                    }
+                }
+            }
+            if (*abort) {
+                if (leader) {  // loads may still be in flight into both CTAs: wait (bounded) for them
+                    for (int k = 0; k < STAGES2; ++k)
+                        if (issued[k]) wait_drain(full0 + 8 * k, issued_ph[k], g.status, g.timeout_ns);
+                } else {  // this CTA cannot observe rank 0's barrier: give its last loads time to land
+                    const uint64_t t0 = ki::globaltimer_ns();
+                    while (ki::globaltimer_ns() - t0 < 200000ull) {
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (leader && lane == 0) {
+            const uint32_t empty_peer0 = map_rank(empty0, 1), tfull_peer0 = map_rank(tfull0, 1);
+            int s = 0, acc = 0;
+            uint32_t ph_full = 0, ph_empty = 1;
+            for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
+                if (!wait_bar(tempty0 + 8 * acc, ph_empty, abort, g.status, g.timeout_ns)) break;
+                tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(acc * TILE2);
+                bool ok = true;
+                for (int kb = 0; kb < blocks; ++kb) {
+                    if (!wait_bar(full0 + 8 * s, ph_full, abort, g.status, g.timeout_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sw = ring + s * STAGE2_BYTES;
+                    const uint64_t wdesc = make_desc(sw, 16, 1024), xdesc = make_desc(sw + W_BYTES, 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < BK / 32; ++k)
+                        mma_i8_pair(d, wdesc + (uint64_t)(2 * k), xdesc + (uint64_t)(2 * k), (kb | k) != 0);
+                    mma_commit_pair(empty0 + 8 * s);       // this CTA's stage is free again
+                    mma_commit_pair(empty_peer0 + 8 * s);  // and the peer's
+                    if (++s == STAGES2) {
+                        s = 0;
+                        ph_full ^= 1;
+                    }
+                }
+                if (!ok) break;
+                mma_commit_pair(tfull0 + 8 * acc);
+                mma_commit_pair(tfull_peer0 + 8 * acc);
+                if (++acc == ACCS2) {
+                    acc = 0;
+                    ph_empty ^= 1;
+                }
+            }
+            mma_commit_pair(drain);  // every MMA issued has finished before TMEM and the rings go
+            wait_drain(drain, 0, g.status, g.timeout_ns);
+        }
+    } else {
+        const int row = (warp & 3) * 32;  // TMEM lanes that this warp may read
+        const int half = (warp - 2) / 4 * (TILE2 / 2);  // and its columns
+        const uint32_t tempty_lead0 = map_rank(tempty0, 0);
+        float* scales = reinterpret_cast<float*>(gbase + RING2_BYTES + 256);
+        int acc = 0;
+        uint32_t ph = 0;
+        for (int tile = pair; tile < tiles; tile += pairs) {
+            int mb, nb;
+            tile2_coords(tile, g.mtiles, g.ntiles, mb, nb);
+            const int m0 = mb * TILE2, n = nb * TILE2 + 128 * (int)rank + row + lane;
+            const bool on = n < g.n;
+            const float sw = on ? g.sw[n] : 0.0f, bias = on && g.bias ? g.bias[n] : 0.0f;
+            // a buffer is written again two tiles later, behind the next tile's barrier, when all have read it
+            float* sa = scales + acc * TILE2;
+            const int mine = (int)threadIdx.x - 64;
+            sa[mine] = m0 + mine < g.m ? g.sa[m0 + mine] : 0.0f;
+            asm volatile("bar.sync 1, %0;" ::"r"(32 * EPI2_WARPS) : "memory");
+            int ok = 0;
+            if (lane == 0) ok = wait_bar(tfull0 + 8 * acc, ph, abort, g.status, g.timeout_ns) ? 1 : 0;
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (ok) {
+                tc_fence_after();
+#pragma unroll 1
+                for (int c0 = half; c0 < half + TILE2 / 2; c0 += 32) {
+                    uint32_t v[32];
+                    KI_TMEM_LD_X32(tmem + ((uint32_t)row << 16) + (uint32_t)(acc * TILE2 + c0), v);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (c0 == half + TILE2 / 2 - 32) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(tempty_lead0 + 8 * acc);
+                    }
+                    if (on)
+                        store_columns(static_cast<O*>(g.c) + (size_t)(m0 + c0) * g.ldc + n, g.ldc, v, sa + c0, sw, bias,
+                                      g.m - m0 - c0);
+                }
+            }
+            if (++acc == ACCS2) {
+                acc = 0;
+                ph ^= 1;
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // neither CTA leaves while the other may still read its shared memory or TMEM
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(ACCS2 * TILE2) : "memory");
+    }
+}
+
+// Tensor maps of both operands with boxes of rows_a and rows_w rows x 128 bytes.
+int encode_operands(ki_ctx* ctx, const GemmArgs& g, CUtensorMap* tA, CUtensorMap* tW, int rows_a, int rows_w) {
+    auto enc = get_encode();
+    if (!enc) return ki::set_error(ctx, KI_ERR_CUDA, "gemm_i8: cuTensorMapEncodeTiled unavailable");
+    // a single row has no stride of its own
+    const uint64_t one = (uint64_t)(g.k + 15) / 16 * 16, lda = g.m > 1 ? g.lda : one, ldw = g.n > 1 ? g.ldw : one;
+    if (!encode_2d(enc, tA, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.a, (uint64_t)g.k, (uint64_t)g.m, lda, BK, rows_a,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
+        !encode_2d(enc, tW, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w, (uint64_t)g.k, (uint64_t)g.n, ldw, BK, rows_w,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
+        return ki::set_error(ctx, KI_ERR_ARG, "gemm_i8: tensor map encoding failed");
+    return KI_OK;
+}
+
+template <class O>
+int launch_pairs(ki_ctx* ctx, GemmArgs& g, cudaStream_t s) {
+    CUtensorMap tA, tW;
+    const int st = encode_operands(ctx, g, &tA, &tW, 128, 128);
+    if (st != KI_OK) return st;
+    auto kern = gemm_i8_pair_kernel<O>;
+    KI_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM2_BYTES));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(THREADS2);
+    cfg.dynamicSmemBytes = SMEM2_BYTES;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (ctx->gemm_i8_pairs == 0) {
+        int nc = 0;
+        cfg.gridDim = dim3(2 * (ctx->sm_count / 2));
+        if (cudaOccupancyMaxActiveClusters(&nc, kern, &cfg) != cudaSuccess || nc < 1) {
+            cudaGetLastError();
+            nc = ctx->sm_count / 2;
+        }
+        ctx->gemm_i8_pairs = nc;
+    }
+    g.ntiles = (g.n + TILE2 - 1) / TILE2;
+    g.mtiles = (g.m + TILE2 - 1) / TILE2;
+    const long long tiles = (long long)g.ntiles * g.mtiles;
+    if (tiles > 0x3fffffffll) return ki::set_error(ctx, KI_ERR_ARG, "gemm_i8: too many tiles");
+    cfg.gridDim = dim3(2 * (unsigned)(tiles < ctx->gemm_i8_pairs ? tiles : ctx->gemm_i8_pairs));
+    KI_CUDA(ctx, cudaLaunchKernelEx(&cfg, kern, tA, tW, g));
+    return ki::check_launch(ctx, "gemm_i8_pair_kernel launch");
+}
+
 template <int BN, class O, bool TMA>
 int launch(ki_ctx* ctx, GemmArgs& g, cudaStream_t s) {
-    using S = Shape<BN>;
+    using S = Shape<BN, TMA>;
     CUtensorMap tA = {}, tW = {};
     if (TMA) {
-        auto enc = get_encode();
-        if (!enc) return ki::set_error(ctx, KI_ERR_CUDA, "gemm_i8: cuTensorMapEncodeTiled unavailable");
-        // a single row has no stride of its own
-        const uint64_t lda = g.m > 1 ? g.lda : (g.k + 15) / 16 * 16, ldw = g.n > 1 ? g.ldw : (g.k + 15) / 16 * 16;
-        if (!encode_2d(enc, &tA, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.a, (uint64_t)g.k, (uint64_t)g.m, lda, BK, BN,
-                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
-            !encode_2d(enc, &tW, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w, (uint64_t)g.k, (uint64_t)g.n, ldw, BK, BM,
-                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
-            return ki::set_error(ctx, KI_ERR_ARG, "gemm_i8: tensor map encoding failed");
+        const int st = encode_operands(ctx, g, &tA, &tW, BN, BM);
+        if (st != KI_OK) return st;
     }
     g.ntiles = (g.n + BM - 1) / BM;
     g.mtiles = (g.m + BN - 1) / BN;
@@ -325,7 +667,7 @@ int launch(ki_ctx* ctx, GemmArgs& g, cudaStream_t s) {
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(tiles * split));
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(TMA ? S::THREADS : THREADS_ROWS);
     cfg.dynamicSmemBytes = S::SMEM_BYTES;
     cfg.stream = s;
     cfg.attrs = attr;
@@ -369,6 +711,9 @@ extern "C" int ki_gemm_i8(ki_ctx* ctx, const int8_t* d_A, size_t lda, const int8
     cudaStream_t s = ki::as_stream(stream);
     return ki::with_float_type(out_dtype, [&](auto t) {
         using O = decltype(t);
+        // pairs where their tiles fill the SMs
+        const long long tiles2 = (long long)((N + TILE2 - 1) / TILE2) * (long long)((M + TILE2 - 1) / TILE2);
+        if (tma && tiles2 >= KI_I8_PAIRS) return launch_pairs<O>(ctx, g, s);
         if (M <= 16) return launch_tma<16, O>(ctx, g, tma, s);
         if (M <= 32) return launch_tma<32, O>(ctx, g, tma, s);
         if (M <= 64) return launch_tma<64, O>(ctx, g, tma, s);

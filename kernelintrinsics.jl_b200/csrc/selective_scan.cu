@@ -15,7 +15,7 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kStepThreads = 256;
 
 struct ScanArgs {
     const void* u;
@@ -440,40 +440,68 @@ __global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ?
     if (chunks > 0) finish(chunks - 1);
 }
 
-// One token per row: row r continues slot slots[r].  LPC lanes share a channel.
-template <class T, int LPC>
-__global__ void __launch_bounds__(kThreads) scan_step_kernel(const ScanArgs a, int tiles) {
-    constexpr int DT = kThreads / LPC;
-    const int r = blockIdx.x / tiles;
+// One token per row: row r continues slot slots[r].  Bound: the states' bytes (one read and one write), so LPC lanes
+// share a channel with K states each (16 bytes and more per access) and take R rows at once: A is read once for them and
+// their states' loads are in flight together.  What is done once per row and channel (the step, the gate) is done
+// by lane r of the group for row r.
+template <class T, int LPC, int K, int R>
+__global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const ScanArgs a, int tiles) {
+    static_assert(LPC >= R, "a lane per row");
+    constexpr int DT = kStepThreads / LPC;
+    const int r0 = (int)(blockIdx.x / tiles) * R;
     const int d = (int)(blockIdx.x % tiles) * DT + (int)threadIdx.x / LPC;
-    const int lane = threadIdx.x % LPC;
-    const int64_t slot = a.seq.slot(r);
-    if (slot < 0) return;
+    const int lane = threadIdx.x % LPC, n0 = lane * K;
     const bool live = d < a.channels;
-    float p = 0.0f, u = 0.0f;
-    if (live) {
-        const int g = d / (a.channels / a.groups);
-        u = ki::to_f32(static_cast<const T*>(a.u)[(size_t)r * a.ldu + d]);
-        float s = ki::to_f32(static_cast<const T*>(a.delta)[(size_t)r * a.ldd + d]);
+    const int n = live ? min(max(a.states - n0, 0), K) : 0;
+    const int g = live ? d / (a.channels / a.groups) : 0;
+
+    int64_t slot[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) slot[r] = r0 + r < a.seq.count ? a.seq.slot(r0 + r) : -1;
+    Raw<float, K> h[R];
+    Raw<T, K> b[R], c[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (slot[r] < 0) continue;
+        h[r].load(a.state + (size_t)slot[r] * a.state_ld + (size_t)d * a.states + n0, a.vec, n);
+        b[r].load(static_cast<const T*>(a.B) + (size_t)(r0 + r) * a.ldb + (size_t)g * a.states + n0, a.vec_b, n);
+        c[r].load(static_cast<const T*>(a.C) + (size_t)(r0 + r) * a.ldc + (size_t)g * a.states + n0, a.vec_c, n);
+    }
+    Raw<float, K> A;
+    A.load(a.A + (size_t)d * a.states + n0, a.vec, n);
+    float s = 0.0f, u = 0.0f, z = 0.0f;  // of row r0 + lane
+    const int row = r0 + lane;
+    const bool mine = lane < R && row < a.seq.count && live;
+    if (mine) {
+        u = ki::to_f32(static_cast<const T*>(a.u)[(size_t)row * a.ldu + d]);
+        s = ki::to_f32(static_cast<const T*>(a.delta)[(size_t)row * a.ldd + d]);
+        if (a.z) z = ki::to_f32(static_cast<const T*>(a.z)[(size_t)row * a.ldz + d]);
         if (a.delta_bias) s += a.delta_bias[d];
         if (a.soft) s = ki::softplus(s);
-        const float su = s * u;
-        float* st = a.state + (size_t)slot * a.state_ld + (size_t)d * a.states;
-        const float* A = a.A + (size_t)d * a.states;
-        const T* B = static_cast<const T*>(a.B) + (size_t)r * a.ldb + (size_t)g * a.states;
-        const T* C = static_cast<const T*>(a.C) + (size_t)r * a.ldc + (size_t)g * a.states;
-        for (int n = lane; n < a.states; n += LPC) {
-            const float h = fmaf(ki::exp2_fast(s * (A[n] * ki::kLog2e)), st[n], su * ki::to_f32(B[n]));
-            st[n] = h;
-            p = fmaf(ki::to_f32(C[n]), h, p);
-        }
     }
+    float y = 0.0f;
 #pragma unroll
-    for (int h = LPC / 2; h >= 1; h /= 2) p += __shfl_xor_sync(0xffffffffu, p, h);
-    if (live && lane == 0) {
-        if (a.D) p = fmaf(a.D[d], u, p);
-        if (a.z) p *= ki::silu(ki::to_f32(static_cast<const T*>(a.z)[(size_t)r * a.ldz + d]));
-        static_cast<T*>(a.y)[(size_t)r * a.ldy + d] = ki::from_f32<T>(p);
+    for (int r = 0; r < R; ++r) {
+        const float sr = __shfl_sync(0xffffffffu, s, r, LPC);
+        const float su = __shfl_sync(0xffffffffu, s * u, r, LPC);
+        float p = 0.0f;
+        if (slot[r] >= 0 && live) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const float v = fmaf(ki::exp2_fast(sr * (A.get(k) * ki::kLog2e)), h[r].get(k), su * ki::to_f32(b[r].get(k)));
+                h[r].w[k] = __float_as_uint(v);
+                if (k < n) p = fmaf(ki::to_f32(c[r].get(k)), v, p);
+            }
+            h[r].store(a.state + (size_t)slot[r] * a.state_ld + (size_t)d * a.states + n0, a.vec, n);
+        }
+#pragma unroll
+        for (int x = LPC / 2; x >= 1; x /= 2) p += __shfl_xor_sync(0xffffffffu, p, x);
+        if (lane == r) y = p;
+    }
+    if (mine && a.seq.slot(row) >= 0) {
+        if (a.D) y = fmaf(a.D[d], u, y);
+        if (a.z) y *= ki::silu(z);
+        static_cast<T*>(a.y)[(size_t)row * a.ldy + d] = ki::from_f32<T>(y);
     }
 }
 
@@ -518,13 +546,38 @@ int launch_scan(ki_ctx* ctx, ScanArgs& a, cudaStream_t s) {
     return launch<T, 32, 8>(ctx, a, s);
 }
 
+template <class T, int LPC, int K, int R>
+int launch_rows(ki_ctx* ctx, ScanArgs& a, cudaStream_t s) {
+    constexpr int DT = kStepThreads / LPC;
+    const long long tiles = (a.channels + DT - 1) / DT;
+    const long long blocks = tiles * ((a.seq.count + R - 1) / R);
+    if (blocks > 0x7fffffffll) return ki::set_error(ctx, KI_ERR_ARG, "selective_scan_step: too many rows");
+    const size_t es = sizeof(T), w = K * es > 16 ? 16 : K * es;
+    const bool one = a.seq.count <= 1;
+    a.vec = a.states % 4 == 0 && ki::aligned(a.A, 16) && ki::rows_aligned(a.state, a.seq.nslots > 1 ? a.state_ld : 0, 4, 16);
+    a.vec_b = (a.groups == 1 || a.states * es % w == 0) && ki::rows_aligned(a.B, one ? 0 : a.ldb, es, w);
+    a.vec_c = (a.groups == 1 || a.states * es % w == 0) && ki::rows_aligned(a.C, one ? 0 : a.ldc, es, w);
+    scan_step_kernel<T, LPC, K, R><<<(unsigned)blocks, kStepThreads, 0, s>>>(a, (int)tiles);
+    return ki::check_launch(ctx, "selective_scan_step launch");
+}
+
+template <class T, int LPC, int K>
+int launch_step_lanes(ki_ctx* ctx, ScanArgs& a, cudaStream_t s) {
+    // several rows per block where that still leaves two blocks for every SM
+    constexpr int DT = kStepThreads / LPC;
+    const long long tiles = (a.channels + DT - 1) / DT;
+    if (LPC >= 4 && tiles * ((a.seq.count + 3) / 4) >= 2ll * ctx->sm_count) return launch_rows<T, LPC, K, LPC >= 4 ? 4 : 1>(ctx, a, s);
+    return launch_rows<T, LPC, K, 1>(ctx, a, s);
+}
+
 template <class T>
 int launch_step(ki_ctx* ctx, ScanArgs& a, cudaStream_t s) {
-    constexpr int LPC = 8, DT = kThreads / LPC;
-    const long long tiles = (a.channels + DT - 1) / DT;
-    if (tiles * a.seq.count > 0x7fffffffll) return ki::set_error(ctx, KI_ERR_ARG, "selective_scan_step: too many rows");
-    scan_step_kernel<T, LPC><<<(unsigned)(tiles * a.seq.count), kThreads, 0, s>>>(a, (int)tiles);
-    return ki::check_launch(ctx, "selective_scan_step launch");
+    if (a.states <= 8) return launch_step_lanes<T, 4, 2>(ctx, a, s);
+    if (a.states <= 16) return launch_step_lanes<T, 4, 4>(ctx, a, s);
+    if (a.states <= 32) return launch_step_lanes<T, 8, 4>(ctx, a, s);
+    if (a.states <= 64) return launch_step_lanes<T, 16, 4>(ctx, a, s);
+    if (a.states <= 128) return launch_step_lanes<T, 32, 4>(ctx, a, s);
+    return launch_step_lanes<T, 32, 8>(ctx, a, s);
 }
 
 int scan(ki_ctx* ctx, const char* what, int dtype, ScanArgs& a, size_t rows, size_t channels, size_t states, size_t groups,

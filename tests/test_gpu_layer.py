@@ -137,7 +137,8 @@ def _check_product(out, a, w, sa, sw, bias, dtype):
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 128, 128), (1, 300, 4096), (2, 129, 48), (15, 64, 1000), (16, 256, 256),
                                    (17, 130, 130), (33, 200, 2064), (48, 1024, 512), (64, 128, 129), (65, 127, 127),
                                    (128, 128, 2048), (129, 257, 255), (200, 700, 640), (256, 512, 384), (300, 2049, 272),
-                                   (513, 1040, 144), (1024, 1024, 256), (1111, 515, 257), (2050, 2304, 128)])
+                                   (513, 1040, 144), (1024, 1024, 256), (1111, 515, 257), (2050, 2304, 128), (2049, 2060, 400),
+                                   (4100, 1030, 1040)])
 def test_int8_gemm(KI, dev, M, N, K):
     import torch
 
