@@ -197,11 +197,10 @@ def context(device: Optional[int] = None) -> Context:
     if device is None:
         device = torch.cuda.current_device()
     key = (threading.get_ident(), int(device))
-    with _ctx_lock:
-        c = _ctx_by_key.get(key)
-        if c is None:
-            c = Context(int(device))
-            _ctx_by_key[key] = c
+    c = _ctx_by_key.get(key)  # only this thread makes the entry
+    if c is None:
+        with _ctx_lock:
+            c = _ctx_by_key[key] = Context(int(device))
     return c
 
 
@@ -836,6 +835,14 @@ def _new(shape: tuple, dtype, like, stream):
         return like.new_empty(shape, dtype=dtype)
 
 
+def _like(x, dtype, stream):
+    """A new tensor of ``x``'s shape (whose rows are contiguous), with contiguous rows that follow each other."""
+    if stream is None:
+        return _torch().empty_like(x, dtype=dtype)
+    with _torch().cuda.stream(stream):
+        return _torch().empty_like(x, dtype=dtype)
+
+
 def _raw_stream(stream, d: int) -> int:
     if stream is not None:
         if stream.device.index != d:
@@ -914,7 +921,7 @@ def quantize_rows(x, out=None, scale=None, stream=None):
     code = _float_code(name, x.dtype)
     ld = _rows(name, "x", x, shape, x.dtype, d)
     if out is None:
-        out, ldq = _new(shape, torch.int8, x, stream), cols
+        out, ldq = _like(x, torch.int8, stream), cols
     else:
         ldq = _rows(name, "out", out, shape, torch.int8, d)
     if scale is None:
@@ -978,7 +985,7 @@ def causal_conv(x, weight, bias=None, state=None, offsets=None, slots=None, init
     ps, state_ld, n, pslots = _state(name, state, width - 1, channels, dtype, d, slots, count)
     silu = _silu(name, activation)
     if out is None:
-        out, ldy = _new(shape, dtype, x, stream), channels
+        out, ldy = _like(x, dtype, stream), channels
     else:
         ldy = _rows(name, "out", out, shape, dtype, d)
     context(d).call("ki_causal_conv", code, x.data_ptr(), ldx, pw, pb, ps, state_ld, n, pslots, flags, at, count,
@@ -1003,7 +1010,7 @@ def causal_conv_step(x, weight, bias=None, state=None, slots=None, activation=No
     ps, state_ld, n, pslots = _state(name, state, width - 1, channels, dtype, d, slots, rows)
     silu = _silu(name, activation)
     if out is None:
-        out, ldy = _new(shape, dtype, x, stream), channels
+        out, ldy = _like(x, dtype, stream), channels
     else:
         ldy = _rows(name, "out", out, shape, dtype, d)
     context(d).call("ki_causal_conv_step", code, x.data_ptr(), ldx, pw, pb, ps, state_ld, n, pslots, out.data_ptr(), ldy,
@@ -1065,7 +1072,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     count, at, flags = _sequences(name, offsets, initial, state, d)
     ps, state_ld, n, pslots = _state(name, state, channels, states, _torch().float32, d, slots, count)
     if out is None:
-        out, ldy = _new(shape, u.dtype, u, stream), channels
+        out, ldy = _like(u, u.dtype, stream), channels
     else:
         ldy = _rows(name, "out", out, shape, u.dtype, d)
     context(d).call("ki_selective_scan", *args, 1 if softplus else 0, ps, state_ld, n, pslots, flags, at, count,
@@ -1085,7 +1092,7 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, soft
         raise _bad(f"{name}: a state is needed")
     ps, state_ld, n, pslots = _state(name, state, channels, states, _torch().float32, d, slots, rows)
     if out is None:
-        out, ldy = _new(shape, u.dtype, u, stream), channels
+        out, ldy = _like(u, u.dtype, stream), channels
     else:
         ldy = _rows(name, "out", out, shape, u.dtype, d)
     context(d).call("ki_selective_scan_step", *args, 1 if softplus else 0, ps, state_ld, n, pslots, out.data_ptr(), ldy,
