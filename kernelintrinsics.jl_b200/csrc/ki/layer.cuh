@@ -26,6 +26,20 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two values to neighbouring elements of a word (16-bit types), lo in the lower half.
+template <class T>
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t narrow2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t narrow2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // V consecutive elements moved with one access of sizeof(T) * V bytes (at most 16).
 template <class T, int V>
 struct alignas(sizeof(T) * V) Vec {
@@ -83,33 +97,30 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
     return r;
 }
 
-// log(1 + e^x) = max(x, 0) + log1p(e), e = e^-|x| <= 1, of two values.  The exponent's product with log2(e) is
-// kept to twice Float32's precision; log1p(e) / e is a polynomial of degree 8, fitted on [0, 1] for the smallest
-// relative error (3e-8; 1.7e-7 with Float32 arithmetic).  No branches, so neighbouring values overlap.
-__device__ __forceinline__ f32x2 softplus2(f32x2 v) {
-    float x0, x1;
-    unpair(x0, x1, v);
-    const f32x2 n = pair(fmaxf(-fabsf(x0), -200.0f), fmaxf(-fabsf(x1), -200.0f));
-    const f32x2 minus = mul2(n, pair(-kLog2e));
-    const f32x2 lo = fma2(n, pair(1.92596299e-8f), fma2(n, pair(kLog2e), minus));
-    float e0, e1;
-    unpair(e0, e1, minus);
-    f32x2 e = pair(exp2_fast(-e0), exp2_fast(-e1));
-    e = fma2(e, mul2(lo, pair(0.693147182f)), e);
-    f32x2 p = fma2(e, pair(0.005232684314250946f), pair(-0.029505198821425438f));
-    p = fma2(e, p, pair(0.07822588831186295f));
-    p = fma2(e, p, pair(-0.13663239777088165f));
-    p = fma2(e, p, pair(0.19106003642082214f));
-    p = fma2(e, p, pair(-0.2484298199415207f));
-    p = fma2(e, p, pair(0.3331909775733948f));
-    p = fma2(e, p, pair(-0.4999949336051941f));
-    p = fma2(e, p, pair(0.9999999403953552f));
-    return fma2(e, p, pair(x0 < 0.0f ? 0.0f : x0, x1 < 0.0f ? 0.0f : x1));  // NaN stays
+// max(x, 0); NaN stays.
+__device__ __forceinline__ float relu(float x) {
+    float y;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+    return y;
 }
+// log(1 + e^x) = max(x, 0) + log1p(e), e = e^-|x| <= 1.  The exponent's product with log2(e) is kept to twice
+// Float32's precision; log1p(e) / e is a polynomial of degree 8, fitted on [0, 1] for the smallest relative error (3e-8;
+// 1.7e-7 with Float32 arithmetic).  No branches, so neighbouring values overlap.
 __device__ __forceinline__ float softplus(float x) {
-    float lo, hi;
-    unpair(lo, hi, softplus2(pair(x)));
-    return lo;
+    const float n = fmaxf(-fabsf(x), -200.0f);
+    const float minus = n * -kLog2e;
+    const float lo = fmaf(n, 1.92596299e-8f, fmaf(n, kLog2e, minus));
+    float e = exp2_fast(-minus);
+    e = fmaf(e, lo * 0.693147182f, e);
+    float p = fmaf(e, 0.005232684314250946f, -0.029505198821425438f);
+    p = fmaf(e, p, 0.07822588831186295f);
+    p = fmaf(e, p, -0.13663239777088165f);
+    p = fmaf(e, p, 0.19106003642082214f);
+    p = fmaf(e, p, -0.2484298199415207f);
+    p = fmaf(e, p, 0.3331909775733948f);
+    p = fmaf(e, p, -0.4999949336051941f);
+    p = fmaf(e, p, 0.9999999403953552f);
+    return fmaf(e, p, relu(x));
 }
 
 // ---- packed sequences ---------------------------------------------------------------------------

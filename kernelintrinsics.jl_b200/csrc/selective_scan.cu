@@ -37,6 +37,7 @@ struct ScanArgs {
     size_t ldy;
     int channels, states, groups;
     bool soft;
+    bool sort;          // the longest sequences first
     bool vec;           // rows of u, delta, z and y are aligned for accesses of a thread's channels
     bool vec_b, vec_c;  // rows of B and C are aligned for accesses of a thread's states
     ki::Sequences seq;
@@ -109,6 +110,15 @@ struct Raw {
             return *reinterpret_cast<const T*>(&h);
         }
     }
+    __device__ __forceinline__ void set(const float (&v)[N]) {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            if constexpr (sizeof(T) == 4)
+                w[i] = __float_as_uint(v[i]);
+            else
+                w[i] = ki::narrow2<T>(v[2 * i], N > 1 ? v[2 * i + (N > 1)] : 0.0f);
+        }
+    }
     __device__ __forceinline__ uint32_t half(int i) const { return (w[i / 2] >> (16 * (i & 1))) & 0xffffu; }
     __device__ __forceinline__ void set(int i, T v) {  // into words that were zero there
         if constexpr (sizeof(T) == 4)
@@ -159,7 +169,7 @@ struct Lane {
     using L = Tile<T, LPC, K>;
     static constexpr int GW = L::GW;
     static constexpr int P = K == 1 ? 1 : K / 2;  // pairs of states (one state: only the first half is used)
-    float A[2 * P], h[2 * P];
+    ki::f32x2 A[P], h[P];
 
     struct In {
         float2 x;
@@ -188,7 +198,9 @@ struct Lane {
                 b = __uint_as_float(in.w[0]), c = __uint_as_float(in.w[1]);
             else
                 ki::unpair(b, c, widen2<T>(in.w[0]));
-            m.a[0] = ki::pair(ki::exp2_fast(in.x.x * A[0]), 0.0f);
+            float a0, a1;
+            ki::unpair(a0, a1, A[0]);
+            m.a[0] = ki::pair(ki::exp2_fast(in.x.x * a0), 0.0f);
             m.add[0] = ki::pair(in.x.y * b, 0.0f);
             m.c[0] = ki::pair(c, 0.0f);
         } else {
@@ -204,7 +216,7 @@ struct Lane {
                     m.c[k / 2] = widen2<T>(in.w[(K + k) / 2]);
                 }
                 float e0, e1;
-                ki::unpair(e0, e1, ki::mul2(s, ki::pair(A[k], A[k + 1])));
+                ki::unpair(e0, e1, ki::mul2(s, A[k / 2]));
                 m.a[k / 2] = ki::pair(ki::exp2_fast(e0), ki::exp2_fast(e1));
                 m.add[k / 2] = ki::mul2(su, b);
             }
@@ -218,15 +230,16 @@ struct Lane {
             ki::unpair(a, hi, m.a[0]);
             ki::unpair(add, hi, m.add[0]);
             ki::unpair(c, hi, m.c[0]);
-            h[0] = fmaf(a, h[0], add);
-            return c * h[0];
+            ki::unpair(lo, hi, h[0]);
+            lo = fmaf(a, lo, add);
+            h[0] = ki::pair(lo, 0.0f);
+            return c * lo;
         } else {
             ki::f32x2 sum = 0;
 #pragma unroll
             for (int k = 0; k < P; ++k) {
-                const ki::f32x2 hh = ki::fma2(m.a[k], ki::pair(h[2 * k], h[2 * k + 1]), m.add[k]);
-                ki::unpair(h[2 * k], h[2 * k + 1], hh);
-                sum = k == 0 ? ki::mul2(m.c[k], hh) : ki::fma2(m.c[k], hh, sum);
+                h[k] = ki::fma2(m.a[k], h[k], m.add[k]);
+                sum = k == 0 ? ki::mul2(m.c[k], h[k]) : ki::fma2(m.c[k], h[k], sum);
             }
             ki::unpair(lo, hi, sum);
             return lo + hi;
@@ -257,6 +270,22 @@ struct Lane {
     }
 };
 
+// The sequence that is rank-th by length, the longest first (equal ones in order): with more blocks than SMs, a long
+// sequence that starts last would run alone at the end.  At most kSort sequences; run by the whole block.
+constexpr int kSort = kLanes + kHelpers;
+__device__ __forceinline__ int longest(const ki::Sequences& q, int rank, int* lengths) {
+    __shared__ int found;
+    const int i = threadIdx.x;
+    const int mine = i < q.count ? max(0, q.begin(i + 1) - q.begin(i)) : 0;
+    lengths[i] = mine;
+    __syncthreads();
+    int before = 0;
+    for (int j = 0; j < q.count; ++j) before += lengths[j] > mine || (lengths[j] == mine && j < i);
+    if (i < q.count && before == rank) found = i;
+    __syncthreads();
+    return found;
+}
+
 template <class T, int LPC, int K>
 __global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ? 2 : 1)
     scan_kernel(const ScanArgs a, int tiles) {
@@ -266,8 +295,9 @@ __global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ?
     typename L::Stage* stage = reinterpret_cast<typename L::Stage*>(smem);
     const ki::Sequences& q = a.seq;
     if (blockIdx.x == 0) q.check(threadIdx.x, kLanes + kHelpers);
-    const int seq = blockIdx.x / (tiles * a.groups);
+    int seq = blockIdx.x / (tiles * a.groups);
     const int rest = blockIdx.x % (tiles * a.groups);
+    if (a.sort) seq = longest(q, seq, reinterpret_cast<int*>(smem));
     const int g = rest / tiles;
     const int per = a.channels / a.groups;
     const int in0 = (rest % tiles) * DT;  // first channel within the group
@@ -286,13 +316,18 @@ __global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ?
         const int dl = threadIdx.x / LPC, ln = threadIdx.x % LPC;
         const bool keep = st && q.continues(seq);
         Lane<T, LPC, K> lane;
-        lane.A[2 * lane.P - 1] = lane.h[2 * lane.P - 1] = 0.0f;
+        float A[2 * lane.P] = {}, h[2 * lane.P] = {};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const bool on = dl < width && ln * K + k < a.states;
             const size_t at = (size_t)(d0 + dl) * a.states + ln * K + k;
-            lane.A[k] = on ? a.A[at] * ki::kLog2e : 0.0f;
-            lane.h[k] = on && keep ? st[at] : 0.0f;
+            A[k] = on ? a.A[at] * ki::kLog2e : 0.0f;
+            h[k] = on && keep ? st[at] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < lane.P; ++k) {
+            asm volatile("mov.b64 %0, {%1, %2};" : "=l"(lane.A[k]) : "f"(A[2 * k]), "f"(A[2 * k + 1]));
+            lane.h[k] = ki::pair(h[2 * k], h[2 * k + 1]);
         }
         __syncthreads();
         for (int i = 0; i < chunks; ++i) {
@@ -302,8 +337,10 @@ __global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ?
         }
         if (st) {
 #pragma unroll
+            for (int k = 0; k < lane.P; ++k) ki::unpair(h[2 * k], h[2 * k + 1], lane.h[k]);
+#pragma unroll
             for (int k = 0; k < K; ++k)
-                if (dl < width && ln * K + k < a.states) st[(size_t)(d0 + dl) * a.states + ln * K + k] = lane.h[k];
+                if (dl < width && ln * K + k < a.states) st[(size_t)(d0 + dl) * a.states + ln * K + k] = h[k];
         }
         return;
     }
@@ -365,12 +402,9 @@ __global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ?
 #pragma unroll
         for (int j = 0; j < VC; j += 2) {
             constexpr int one = VC > 1 ? 1 : 0;
-            ki::f32x2 x = ki::add2(ki::pair(ki::to_f32(now.delta.get(j)), ki::to_f32(now.delta.get(j + one))),
-                                   ki::pair(bias[j], bias[j + one]));
-            if (a.soft) x = ki::softplus2(x);
-            float x0, x1, v0, v1;
-            ki::unpair(x0, x1, x);
-            ki::unpair(v0, v1, ki::mul2(x, ki::pair(ki::to_f32(now.u.get(j)), ki::to_f32(now.u.get(j + one)))));
+            float x0 = ki::to_f32(now.delta.get(j)) + bias[j], x1 = ki::to_f32(now.delta.get(j + one)) + bias[j + one];
+            if (a.soft) x0 = ki::softplus(x0), x1 = ki::softplus(x1);
+            const float v0 = x0 * ki::to_f32(now.u.get(j)), v1 = x1 * ki::to_f32(now.u.get(j + one));
             step[j] = make_float2(x0, v0);
             if (one) step[j + one] = make_float2(x1, v1);
         }
@@ -407,19 +441,20 @@ __global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ?
         if (i * kTime + t >= len || n == 0) return;
         const size_t row = (size_t)b0 + (size_t)i * kTime + t;
         typename L::Stage& s = stage[i & 1];
-        Raw<T, VC> out = {};
+        float v[VC];
 #pragma unroll
         for (int j = 0; j < VC; ++j) {
-            float v = 0.0f;
+            v[j] = 0.0f;
 #pragma unroll
             for (int k = 0; k < LPC / 4; ++k) {
                 const float4 p = s.part[L::part_at(t, (c0 + j) * (LPC / 4) + k)];
-                v += (p.x + p.y) + (p.z + p.w);
+                v[j] += (p.x + p.y) + (p.z + p.w);
             }
-            if (a.D) v = fmaf(skip[j], ki::to_f32(u0.get(j)), v);
-            if (z) v *= ki::silu(ki::to_f32(z0.get(j)));
-            out.set(j, ki::from_f32<T>(v));
+            if (a.D) v[j] = fmaf(skip[j], ki::to_f32(u0.get(j)), v[j]);
+            if (z) v[j] *= ki::silu(ki::to_f32(z0.get(j)));
         }
+        Raw<T, VC> out;
+        out.set(v);
         out.store(y + row * a.ldy, a.vec, n);
     };
 
@@ -522,6 +557,7 @@ int launch(ki_ctx* ctx, ScanArgs& a, cudaStream_t s) {
     a.vec_b = whole && ki::rows_aligned(a.B, one ? 0 : a.ldb, es, wv);
     a.vec_c = whole && ki::rows_aligned(a.C, one ? 0 : a.ldc, es, wv);
     constexpr int smem = 2 * sizeof(typename L::Stage);
+    a.sort = a.seq.count > 1 && a.seq.count <= kSort && blocks > ctx->sm_count;
     auto kern = scan_kernel<T, LPC, K>;
     KI_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     kern<<<(unsigned)blocks, kLanes + kHelpers, smem, s>>>(a, (int)tiles);
@@ -646,7 +682,7 @@ extern "C" int ki_selective_scan(ki_ctx* ctx, int dtype, const void* d_u, size_t
         return ki::set_error(ctx, KI_ERR_ARG, "selective_scan: too many sequences or slots");
     if (!d_offsets && seqs != 1) return ki::set_error(ctx, KI_ERR_ARG, "selective_scan: several sequences need offsets");
     ScanArgs a{d_u, ldu, d_delta, ldd, d_A, d_B, ldb, d_C, ldc, d_D, d_z, ldz, d_delta_bias, d_state, state_ld, d_y, ldy,
-               0, 0, 0, softplus != 0, false, false, false, {d_offsets, d_slots, d_initial, (int)seqs, 0, (int64_t)slots, nullptr}};
+               0, 0, 0, softplus != 0, false, false, false, false, {d_offsets, d_slots, d_initial, (int)seqs, 0, (int64_t)slots, nullptr}};
     return scan(ctx, "selective_scan", dtype, a, tokens, channels, states, groups, false, stream);
 }
 
@@ -661,6 +697,6 @@ extern "C" int ki_selective_scan_step(ki_ctx* ctx, int dtype, const void* d_u, s
         return ki::set_error(ctx, KI_ERR_ARG, "selective_scan_step: too many rows or slots");
     if (!d_state) return ki::set_error(ctx, KI_ERR_ARG, "selective_scan_step: null pointer");
     ScanArgs a{d_u, ldu, d_delta, ldd, d_A, d_B, ldb, d_C, ldc, d_D, d_z, ldz, d_delta_bias, d_state, state_ld, d_y, ldy,
-               0, 0, 0, softplus != 0, false, false, false, {nullptr, d_slots, nullptr, (int)rows, 0, (int64_t)slots, nullptr}};
+               0, 0, 0, softplus != 0, false, false, false, false, {nullptr, d_slots, nullptr, (int)rows, 0, (int64_t)slots, nullptr}};
     return scan(ctx, "selective_scan_step", dtype, a, rows, channels, states, groups, true, stream);
 }
