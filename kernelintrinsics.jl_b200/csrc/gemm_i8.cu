@@ -85,60 +85,68 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t wdesc, uint64_t
         : "memory");
 }
 
-// 16 rows of a matrix, a K block at a time, loaded by one warp from rows that start at any byte.  Lane l takes the
-// 4-byte word l of every row, and lane r word 32 of row r; a byte shift by the row's misalignment (between neighbouring
-// lanes' words) gives the row's bytes.  Rows r, r + 4, ... share their misalignment.  Only words that hold a byte of a
-// row are read, and what lies behind the rows' end or the last row is zero.  Whole blocks of existing rows, nearly
-// all, take a path without those tests.
+// 16 rows of a matrix, a K block at a time, loaded by one warp from rows that start at any byte.  Eight lanes share a
+// row and load its 16-byte words, as they lie aligned in memory, four rows at once.  A lane's 16 bytes of the block are
+// then its word and the next one, shifted by the row's misalignment; the word behind the last lane's is the first of the
+// next block, which is loaded by then.  Only words that hold a byte of a row are read; what lies behind the rows' end is
+// zero, and rows that do not exist hold anything finite, since their outputs are not stored.
 struct Rows {
-    static constexpr int N = 16;
-    const int8_t* x;  // the first row
-    size_t ld;
-    int rows;         // that exist
-    int k;
+    static constexpr int N = 16, G = N / 4;
+    const int8_t* x;  // this lane's word of its first row (aligned to 16 bytes), K block 0
+    size_t step;      // bytes from a row to the fourth after it
+    int rows;         // rows of this lane's that exist: its own, and every fourth after it
+    int k;            // bytes of a row that exist, counted from x's row's start
     int lane;
-    uint32_t off[4];  // misalignment of rows 0 to 3
+    uint32_t off[G];  // misalignment of this lane's rows
     struct Words {
-        uint32_t w[N], last;
+        uint4 v[G];
     };
-    __device__ __forceinline__ Rows(const int8_t* base, size_t ld_, int row0, int end, int k_, int lane_)
-        : x(base + (size_t)row0 * ld_), ld(ld_), rows(min(end - row0, N)), k(k_), lane(lane_) {
+    __device__ __forceinline__ Rows(const int8_t* base, size_t ld, int row0, int end, int k_, int lane_) : k(k_), lane(lane_) {
+        const int r = lane >> 3;
+        const int8_t* p = base + (size_t)(row0 + r) * ld;
+        x = p + 16 * (lane & 7);
+        step = 4 * ld;
+        rows = (end - row0 - r + 3) / 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) off[j] = (uint32_t)((uintptr_t)x + j * ld) & 3;  // the same in every K block
+        for (int g = 0; g < G; ++g) off[g] = (uint32_t)(uintptr_t)(p + g * step) & 15;  // the same in every K block
     }
-    __device__ __forceinline__ void load(Words& v, int k0) const {
-        const int8_t* p = x + k0;
-        const int bytes = min(k - k0, BK);
-        if (rows == N && bytes == BK) {
-            const int8_t* q[4];
+    // The words of the block that starts with byte k0 of the rows (k0 may lie behind their end, and k is positive).
+    __device__ __forceinline__ void load(Words& w, int k0) const {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) q[j] = p + j * ld - off[j] + 4 * lane;
-#pragma unroll
-            for (int r = 0; r < N; ++r) {
-                v.w[r] = __ldg(reinterpret_cast<const uint32_t*>(q[r & 3]));
-                q[r & 3] += 4 * ld;
-            }
-        } else {
-#pragma unroll
-            for (int r = 0; r < N; ++r)
-                v.w[r] = r < rows && 4 * lane < (int)off[r & 3] + bytes
-                             ? __ldg(reinterpret_cast<const uint32_t*>(p + r * ld - off[r & 3]) + lane)
-                             : 0u;
+        for (int g = 0; g < G; ++g) {
+            w.v[g] = make_uint4(0, 0, 0, 0);
+            if (g < rows && 16 * (lane & 7) < (int)off[g] + k - k0)
+                w.v[g] = __ldg(reinterpret_cast<const uint4*>(x + g * step + k0 - off[g]));
         }
-        const uint32_t o = (uint32_t)((uintptr_t)x + lane * ld) & 3;
-        v.last = lane < rows && BK < (int)o + bytes ? __ldg(reinterpret_cast<const uint32_t*>(p + lane * ld - o) + 32) : 0u;
     }
-    // To shared memory at dst, as a TMA tile with the 128-byte swizzle: row r at 128 r, its 16-byte pieces exchanged by r mod 8.
-    __device__ __forceinline__ void store(const Words& v, uint32_t dst, int k0) const {
-        const int left = min(max(k - k0 - 4 * lane, 0), 4);  // bytes of this lane's word
-        const uint32_t mask = left == 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
+    // To shared memory at dst, as a TMA tile with the 128-byte swizzle: row r at 128 r, its 16-byte pieces exchanged by
+    // r mod 8.
+    __device__ __forceinline__ void store(const Words& w, const Words& next, uint32_t dst, int k0) const {
+        const int j = lane & 7, from = (lane & ~7) | ((j + 1) & 7);
 #pragma unroll
-        for (int r = 0; r < N; ++r) {
-            const uint32_t end = __shfl_sync(0xffffffffu, v.last, r);
-            uint32_t next = __shfl_down_sync(0xffffffffu, v.w[r], 1);
-            if (lane == 31) next = end;
-            const uint32_t b = __funnelshift_r(v.w[r], next, 8 * off[r & 3]) & mask;
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + (uint32_t)(r * 128 + ((4 * lane) ^ ((r & 7) << 4)))), "r"(b)
+        for (int g = 0; g < G; ++g) {
+            uint32_t a[8] = {w.v[g].x, w.v[g].y, w.v[g].z, w.v[g].w};
+            const uint32_t n[4] = {next.v[g].x, next.v[g].y, next.v[g].z, next.v[g].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[4 + i] = __shfl_sync(0xffffffffu, j == 0 ? n[i] : a[i], from);
+            // left by whole words, then by bytes
+            const bool one = off[g] & 4, two = off[g] & 8;
+#pragma unroll
+            for (int i = 0; i < 7; ++i) a[i] = one ? a[i + 1] : a[i];
+#pragma unroll
+            for (int i = 0; i < 5; ++i) a[i] = two ? a[i + 2] : a[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = __funnelshift_r(a[i], a[i + 1], 8 * (off[g] & 3));
+            if (k - k0 < BK) {  // bytes behind the end
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int left = min(max(k - k0 - 16 * j - 4 * i, 0), 4);
+                    a[i] &= left == 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
+                }
+            }
+            const int r = (lane >> 3) + 4 * g;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)(r * 128 + ((j ^ (r & 7)) << 4))),
+                         "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3])
                          : "memory");
         }
     }
@@ -261,19 +269,19 @@ __global__ void __launch_bounds__(TMA ? Shape<BN, TMA>::THREADS : THREADS_ROWS, 
             wait_drain(tfull, 0, g.status, g.timeout_ns);
         }
     } else if (!TMA && warp >= 2) {
-        // W's 128 rows, then A's BN, 16 to a warp; a block's loads are in flight while the one before it is stored
+        // W's 128 rows, then A's BN, 16 to a warp
         static_assert(BM + BN <= Rows::N * LOADERS && BN % Rows::N == 0, "16 rows per warp");
         const int r0 = Rows::N * (warp - 2);
-        const bool some = r0 < BM + BN, isw = r0 < BM;
+        const bool some = r0 < BM + BN && kb0 < kb1, isw = r0 < BM;  // without an inner dimension there is nothing to read
         const Rows rows(isw ? g.w : g.a, isw ? g.ldw : g.lda, isw ? n0 + r0 : m0 + r0 - BM, isw ? g.n : min(g.m, m0 + BN),
                         g.k, lane);
         int s = 0;
         uint32_t ph = 1;
-        auto put = [&](const Rows::Words& v, int kb) {
+        auto put = [&](const Rows::Words& v, const Rows::Words& behind, int kb) {
             int ok = 0;
             if (lane == 0) ok = wait_bar(empty0 + 8 * s, ph, abort, g.status, g.timeout_ns) ? 1 : 0;
             if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
-            if (some) rows.store(v, ring + s * S::STAGE_BYTES + r0 * BK, kb * BK);
+            if (some) rows.store(v, behind, ring + s * S::STAGE_BYTES + r0 * BK, kb * BK);
             ki::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(full0 + 8 * s);
@@ -283,13 +291,20 @@ __global__ void __launch_bounds__(TMA ? Shape<BN, TMA>::THREADS : THREADS_ROWS, 
             }
             return true;
         };
-        Rows::Words even, odd;
-        if (some && kb0 < kb1) rows.load(even, kb0 * BK);
-        for (int kb = kb0; kb < kb1; kb += 2) {
-            if (some && kb + 1 < kb1) rows.load(odd, (kb + 1) * BK);
-            if (!put(even, kb) || kb + 1 == kb1) break;
-            if (some && kb + 2 < kb1) rows.load(even, (kb + 2) * BK);
-            if (!put(odd, kb + 1)) break;
+        // three blocks in turn: one is stored, the next has to be there, the one after it is in flight
+        Rows::Words w0, w1, w2;
+        auto load = [&](Rows::Words& w, int kb) {
+            if (some) rows.load(w, kb * BK);
+        };
+        load(w0, kb0);
+        load(w1, kb0 + 1);
+        for (int kb = kb0; kb < kb1; kb += 3) {
+            load(w2, kb + 2);
+            if (!put(w0, w1, kb) || kb + 1 >= kb1) break;
+            load(w0, kb + 3);
+            if (!put(w1, w2, kb + 1) || kb + 2 >= kb1) break;
+            load(w1, kb + 4);
+            if (!put(w2, w0, kb + 2)) break;
         }
     }
     __syncwarp();
