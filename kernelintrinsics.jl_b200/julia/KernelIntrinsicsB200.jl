@@ -23,6 +23,7 @@ export get_warpsize, devices, deviceid, context, check_device,
        warpreduce_scan!, warpreduce_scan_host!, warpreduce_scan_noalloc!, accumulate_ki!, accumulate_rows_ki!,
        vote_compact, filter_ki, count_ki,
        vcopy!, vcopy2d!, vcopy_strided!, fp8_gemm!,
+       quantize_rows!, int8_gemm!, causal_conv!, causal_conv_step!, selective_scan!, selective_scan_step!,
        Comm, comm_id, comms, sum_sharded, cumsum_sharded!, cumsum_sharded_host!, findall_sharded, shard_range,
        abort!
 
@@ -338,6 +339,123 @@ function fp8_gemm!(C::CuMatrix{Float32}, A::CuMatrix{UInt8}, B::CuMatrix{UInt8};
                      (Ptr{Cvoid}, CuPtr{UInt8}, CuPtr{UInt8}, CuPtr{Float32}, Cint, Cint, Cint, Float32, Float32, Ptr{Cvoid}),
                      c, A, B, C, M, N, K, sa, sb, _stream()))
     return C
+end
+
+# ---- operators of a state-space layer served in 8 bits -----------------------------------------
+# No counterpart in the reference.  Tokens are columns: a row-major tokens x channels matrix of the ABI is a
+# channels x tokens Julia matrix.  Elements are Float32, Float16 or BFloat16; offsets and slot numbers are device
+# arrays of 0-based Int32, as at the ABI.
+_ft(::Type{T}) where {T} = T === Float32 ? Cint(8) : T === Float16 ? Cint(10) : nameof(T) === :BFloat16 ? Cint(11) :
+                           throw(ArgumentError("Float32, Float16 or BFloat16 elements, not $T"))
+function _opt(::Type{T}, x) where {T}
+    x === nothing && return CuPtr{T}(0)
+    eltype(x) === T || (T === UInt8 && eltype(x) === Bool) || throw(ArgumentError("elements of type $T, not $(eltype(x))"))
+    return CuPtr{T}(UInt(pointer(x)))
+end
+function _ld(x)  # elements from column to column
+    x === nothing && return 0
+    stride(x, 1) == 1 || throw(ArgumentError("columns must be contiguous"))
+    return stride(x, 2)
+end
+
+"int8 columns of `x` and their scales: scale = max|x[:, t]| * (1/127), q = rint(x / scale), ties to even."
+function quantize_rows!(q::CuMatrix{Int8}, scale::CuVector{Float32}, x::StridedCuMatrix{T}) where {T}
+    size(q) == size(x) && length(scale) == size(x, 2) || throw(DimensionMismatch("quantize_rows!"))
+    _call(c -> ccall((:ki_quantize_rows, libki), Cint,
+                     (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, Csize_t, Csize_t, CuPtr{Int8}, Csize_t, CuPtr{Float32}, Ptr{Cvoid}),
+                     c, _ft(T), pointer(x), size(x, 2), size(x, 1), _ld(x), q, _ld(q), scale, _stream()))
+    return q, scale
+end
+"""C[n, m] = (sum_k A[k, m] W[k, n]) * sa[m] * sw[n] + bias[n] with exact Int32 sums: A (K x tokens), W (K x channels),
+C (channels x tokens)."""
+function int8_gemm!(C::StridedCuMatrix{T}, A::StridedCuMatrix{Int8}, W::StridedCuMatrix{Int8}, sa::CuVector{Float32},
+                    sw::CuVector{Float32}; bias = nothing) where {T}
+    K, M = size(A); N = size(W, 2)
+    size(W, 1) == K && size(C) == (N, M) && length(sa) == M && length(sw) == N || throw(DimensionMismatch("int8_gemm!"))
+    bias === nothing || length(bias) == N || throw(DimensionMismatch("int8_gemm!"))
+    _call(c -> ccall((:ki_gemm_i8, libki), Cint,
+                     (Ptr{Cvoid}, CuPtr{Int8}, Csize_t, CuPtr{Int8}, Csize_t, CuPtr{Float32}, CuPtr{Float32}, CuPtr{Float32},
+                      Cint, CuPtr{T}, Csize_t, Csize_t, Csize_t, Csize_t, Ptr{Cvoid}),
+                     c, pointer(A), _ld(A), pointer(W), _ld(W), sa, sw, _opt(Float32, bias), _ft(T), pointer(C),
+                     _ld(C), M, N, K, _stream()))
+    return C
+end
+# A cache of states: a x b x slots, and the sequences of packed tokens (columns).
+function _cache(state, a, b, slots, count, name)
+    state === nothing && return (0, 0)
+    size(state)[1:2] == (a, b) || throw(DimensionMismatch(name))
+    strides(state)[1:2] == (1, a) || throw(ArgumentError("$name: every slot of the state must be contiguous"))
+    slots === nothing ? size(state, 3) >= count : length(slots) == count || throw(DimensionMismatch(name))
+    return (stride(state, 3), size(state, 3))
+end
+_sequences(offsets) = offsets === nothing ? 1 : length(offsets) - 1
+"""Causal depthwise convolution of packed sequences: x, y (channels x tokens), w (width x channels), state
+(channels x (width-1) x slots), offsets (sequences + 1)."""
+function causal_conv!(y::StridedCuMatrix{T}, x::StridedCuMatrix{T}, w::CuMatrix{T}; bias = nothing, state = nothing,
+                      offsets = nothing, slots = nothing, initial = nothing, silu::Bool = false) where {T}
+    D, n = size(x); W = size(w, 1); count = _sequences(offsets)
+    size(y) == size(x) && size(w, 2) == D || throw(DimensionMismatch("causal_conv!"))
+    sld, ns = _cache(state, D, W - 1, slots, count, "causal_conv!")
+    _call(c -> ccall((:ki_causal_conv, libki), Cint,
+                     (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, CuPtr{T}, CuPtr{T}, Csize_t, Csize_t, CuPtr{Int32},
+                      CuPtr{UInt8}, CuPtr{Int32}, Csize_t, CuPtr{T}, Csize_t, Csize_t, Csize_t, Cint, Cint, Ptr{Cvoid}),
+                     c, _ft(T), pointer(x), _ld(x), w, _opt(T, bias), _opt(T, state), sld, ns, _opt(Int32, slots),
+                     _opt(UInt8, initial), _opt(Int32, offsets), count, pointer(y), _ld(y), n, D, W, silu, _stream()))
+    return y
+end
+"One token per column: column r continues slot `slots[r]` of the state."
+function causal_conv_step!(y::StridedCuMatrix{T}, x::StridedCuMatrix{T}, w::CuMatrix{T}, state::StridedCuArray{T,3}; bias = nothing,
+                           slots = nothing, silu::Bool = false) where {T}
+    D, n = size(x); W = size(w, 1)
+    size(y) == size(x) && size(w, 2) == D || throw(DimensionMismatch("causal_conv_step!"))
+    sld, ns = _cache(state, D, W - 1, slots, n, "causal_conv_step!")
+    _call(c -> ccall((:ki_causal_conv_step, libki), Cint,
+                     (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, CuPtr{T}, CuPtr{T}, Csize_t, Csize_t, CuPtr{Int32},
+                      CuPtr{T}, Csize_t, Csize_t, Csize_t, Cint, Cint, Ptr{Cvoid}),
+                     c, _ft(T), pointer(x), _ld(x), w, _opt(T, bias), _opt(T, state), sld, ns, _opt(Int32, slots),
+                     pointer(y), _ld(y), n, D, W, silu, _stream()))
+    return y
+end
+function _scan_sizes(u, delta, A, B, C, z, groups, y, name)
+    D, n = size(u); N = size(A, 1)
+    size(y) == size(u) && size(delta) == size(u) && size(A, 2) == D && size(B) == (groups * N, n) && size(C) == size(B) &&
+        (z === nothing || size(z) == size(u)) || throw(DimensionMismatch(name))
+    return D, n, N
+end
+"""Selective scan of packed sequences: u, delta, z, y (channels x tokens), A (states x channels), B, C
+(groups*states x tokens), state (states x channels x slots, Float32)."""
+function selective_scan!(y::StridedCuMatrix{T}, u::StridedCuMatrix{T}, delta::StridedCuMatrix{T}, A::CuMatrix{Float32},
+                         B::StridedCuMatrix{T}, C::StridedCuMatrix{T}; D = nothing, z = nothing, delta_bias = nothing,
+                         softplus::Bool = false, state = nothing, offsets = nothing, slots = nothing, initial = nothing,
+                         groups::Integer = 1) where {T}
+    d, n, N = _scan_sizes(u, delta, A, B, C, z, groups, y, "selective_scan!")
+    count = _sequences(offsets)
+    sld, ns = _cache(state, N, d, slots, count, "selective_scan!")
+    _call(c -> ccall((:ki_selective_scan, libki), Cint,
+                     (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{T},
+                      Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{Float32}, Cint, CuPtr{Float32}, Csize_t, Csize_t,
+                      CuPtr{Int32}, CuPtr{UInt8}, CuPtr{Int32}, Csize_t, CuPtr{T}, Csize_t, Csize_t, Csize_t, Csize_t,
+                      Csize_t, Ptr{Cvoid}),
+                     c, _ft(T), pointer(u), _ld(u), pointer(delta), _ld(delta), A, pointer(B), _ld(B),
+                     pointer(C), _ld(C), _opt(Float32, D), _opt(T, z), _ld(z), _opt(Float32, delta_bias), softplus,
+                     _opt(Float32, state), sld, ns, _opt(Int32, slots), _opt(UInt8, initial), _opt(Int32, offsets), count,
+                     pointer(y), _ld(y), n, d, N, groups, _stream()))
+    return y
+end
+"One token per column: column r continues slot `slots[r]` of the state."
+function selective_scan_step!(y::StridedCuMatrix{T}, u::StridedCuMatrix{T}, delta::StridedCuMatrix{T}, A::CuMatrix{Float32},
+                              B::StridedCuMatrix{T}, C::StridedCuMatrix{T}, state::StridedCuArray{Float32,3}; D = nothing, z = nothing,
+                              delta_bias = nothing, softplus::Bool = false, slots = nothing, groups::Integer = 1) where {T}
+    d, n, N = _scan_sizes(u, delta, A, B, C, z, groups, y, "selective_scan_step!")
+    sld, ns = _cache(state, N, d, slots, n, "selective_scan_step!")
+    _call(c -> ccall((:ki_selective_scan_step, libki), Cint,
+                     (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{T},
+                      Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{Float32}, Cint, CuPtr{Float32}, Csize_t, Csize_t,
+                      CuPtr{Int32}, CuPtr{T}, Csize_t, Csize_t, Csize_t, Csize_t, Csize_t, Ptr{Cvoid}),
+                     c, _ft(T), pointer(u), _ld(u), pointer(delta), _ld(delta), A, pointer(B), _ld(B),
+                     pointer(C), _ld(C), _opt(Float32, D), _opt(T, z), _ld(z), _opt(Float32, delta_bias), softplus,
+                     _opt(Float32, state), sld, ns, _opt(Int32, slots), pointer(y), _ld(y), n, d, N, groups, _stream()))
+    return y
 end
 
 # ---- several GPUs: communicators and sharded operations ---------------------------------------

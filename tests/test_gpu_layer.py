@@ -186,6 +186,10 @@ def test_int8_gemm_extremes(KI, dev):
     with pytest.raises(KI.KIArgumentError):
         KI.int8_gemm(torch.zeros(1, K + 1, dtype=torch.int8, device=dev), torch.zeros(1, K + 1, dtype=torch.int8, device=dev),
                      one[:1].clone(), one[:1].clone())
+    # (its rows have a stride of one, and may start anywhere)
+    e = torch.empty(5, 3, dtype=torch.int8, device=dev)[:, 1:1]
+    assert torch.equal(KI.int8_gemm(e, torch.empty(7, 2, dtype=torch.int8, device=dev)[:, 2:], torch.ones(5, device=dev),
+                                    torch.ones(7, device=dev), dtype=torch.float32), torch.zeros(5, 7, device=dev))
     e = torch.empty(5, 0, dtype=torch.int8, device=dev)
     bias = torch.arange(7.0, device=dev)
     sc = torch.ones(7, device=dev)
@@ -405,6 +409,38 @@ def test_selective_scan_states(KI, dev, states):
     c, state, slots, initial = _scan_case(states, 200, 3, 24, states, 2, "float32", dev, soft=False, gate=False)
     c["D"] = None
     _scan_check(KI, dev, c, state, slots, initial, offsets)
+
+
+@pytest.mark.parametrize("n,channels", [(12, 700), (256, 40), (300, 40)])
+def test_selective_scan_longest_first(KI, dev, n, channels):
+    """More blocks than SMs: sequences are taken by length, equal ones and empty ones among them."""
+    import torch
+
+    lengths = torch.randint(0, 9, (n,), generator=_rng(n)).tolist()
+    lengths[n // 2] = 40
+    offsets = [0] + np.cumsum(lengths).tolist()
+    c, state, slots, initial = _scan_case(n, offsets[-1] + 3, n, channels, 16, 1, "float32", dev)
+    slots[3] = -1
+    _scan_check(KI, dev, c, state, slots, initial, offsets)
+
+
+def test_one_slot_named_twice(KI, dev):
+    """Not allowed; the call still only touches that slot."""
+    import torch
+
+    offsets = torch.tensor([0, 3, 50], dtype=torch.int32, device=dev)
+    twice = torch.tensor([2, 2], dtype=torch.int32, device=dev)
+    x, w, bias, state, *_ = _conv_case(1, [0, 3, 50], 64, 4, "float32", dev, more=0)
+    c, hs, _, _ = _scan_case(4, 50, 2, 64, 16, 1, "float32", dev)
+    keep, hkeep = state.clone(), hs.clone()
+    KI.causal_conv(x, w, bias, state=state, offsets=offsets, slots=twice)
+    KI.causal_conv_step(x[:2], w, bias, state=state, slots=twice)
+    KI.selective_scan(**c, state=hs, offsets=offsets, slots=twice)
+    step = {k: v[:2] if k in ("u", "delta", "B", "C", "z") else v for k, v in c.items()}
+    KI.selective_scan_step(**step, state=hs, slots=twice)
+    KI.context(0).check()
+    rest = [i for i in range(state.shape[0]) if i != 2]
+    assert torch.equal(state[rest], keep[rest]) and torch.equal(hs[rest], hkeep[rest])
 
 
 def test_selective_scan_padding_and_strides(KI, dev):
