@@ -17,6 +17,8 @@
 //
 // A row stays in registers between the two passes: TPR threads hold VPT vectors each.  Rows longer
 // than that are read twice (the second time from L2).
+#include <type_traits>
+
 #include "ki/layer.cuh"
 
 namespace {
@@ -30,6 +32,17 @@ __device__ __forceinline__ int8_t divided(float x, float scale) {
     return (int8_t)min(max(__float2int_rn(__fdiv_rn(x, scale)), -127), 127);  // NaN: 0
 }
 
+// The larger of m and |x| in either half; NaN stays.
+template <class T>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t x) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value)
+        asm("{\n\t.reg .b32 a;\n\tabs.f16x2 a, %2;\n\tmax.NaN.f16x2 %0, %1, a;\n\t}" : "=r"(r) : "r"(m), "r"(x));
+    else
+        asm("{\n\t.reg .b32 a;\n\tabs.bf16x2 a, %2;\n\tmax.NaN.bf16x2 %0, %1, a;\n\t}" : "=r"(r) : "r"(m), "r"(x));
+    return r;
+}
+
 // The largest |x| so far and of a vector, as bits: of a Float32, or of two 16-bit elements in either half.
 template <class T, int EV>
 __device__ __forceinline__ uint32_t abs_bits(const ki::Vec<T, EV>& v, uint32_t m) {
@@ -41,7 +54,7 @@ __device__ __forceinline__ uint32_t abs_bits(const ki::Vec<T, EV>& v, uint32_t m
     } else {
         const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
 #pragma unroll
-        for (int e = 0; e < EV / 2; ++e) m = __vmaxu2(m, w[e] & 0x7fff7fffu);
+        for (int e = 0; e < EV / 2; ++e) m = max_abs2<T>(m, w[e]);
     }
     return m;
 }

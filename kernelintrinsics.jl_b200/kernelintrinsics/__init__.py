@@ -799,6 +799,13 @@ def _float_code(name: str, dtype) -> int:
     return code
 
 
+def _index(name: str, t) -> int:
+    d = t.get_device()
+    if d < 0:
+        raise _bad(f"{name}: tensors must be on a CUDA device (there is no CPU path)")
+    return d
+
+
 def _refuse(name: str, what: str, t, shape: tuple, dtype, d: int, how: str):
     if t.get_device() != d:
         raise _bad(f"{name}: {what} is on {t.device}, not on cuda:{d}")
@@ -916,7 +923,7 @@ def quantize_rows(x, out=None, scale=None, stream=None):
     Returns (out, scale): int8 of x's shape, Float32 per row."""
     torch = _torch()
     name = "quantize_rows"
-    d = _dev(x)
+    d = _index(name, x)
     rows, cols = shape = _matrix(name, "x", x)
     code = _float_code(name, x.dtype)
     ld = _rows(name, "x", x, shape, x.dtype, d)
@@ -926,7 +933,9 @@ def quantize_rows(x, out=None, scale=None, stream=None):
         ldq = _rows(name, "out", out, shape, torch.int8, d)
     if scale is None:
         scale = _new((rows,), torch.float32, x, stream)
-    ps = _flat(name, "scale", scale, (rows,), torch.float32, d)
+        ps = scale.data_ptr()
+    else:
+        ps = _flat(name, "scale", scale, (rows,), torch.float32, d)
     context(d).call("ki_quantize_rows", code, x.data_ptr(), rows, cols, ld, out.data_ptr(), ldq, ps,
                     _raw_stream(stream, d))
     return out, scale
@@ -938,7 +947,7 @@ def int8_gemm(A, W, scale_a, scale_w, bias=None, out=None, dtype=None, stream=No
     token and per channel, Float32 ``bias`` or None.  ``out`` has ``dtype`` (bfloat16 unless given)."""
     torch = _torch()
     name = "int8_gemm"
-    d = _dev(A)
+    d = _index(name, A)
     M, K = shape = _matrix(name, "A", A)
     N = _matrix(name, "W", W)[0]
     if dtype is None:
@@ -973,7 +982,7 @@ def causal_conv(x, weight, bias=None, state=None, offsets=None, slots=None, init
     are not written (a new output holds anything there).  A bad offset or slot number is reported by
     ``Context.check``."""
     name = "causal_conv"
-    d = _dev(x)
+    d = _index(name, x)
     tokens, channels = shape = _matrix(name, "x", x)
     width = _matrix(name, "weight", weight)[1]
     dtype = x.dtype
@@ -997,7 +1006,7 @@ def causal_conv_step(x, weight, bias=None, state=None, slots=None, activation=No
     """One token per row: row r of ``x`` (rows x channels) continues state slot ``slots[r]`` (None: slot r), which
     is updated; the arguments are those of ``causal_conv``."""
     name = "causal_conv_step"
-    d = _dev(x)
+    d = _index(name, x)
     rows, channels = shape = _matrix(name, "x", x)
     width = _matrix(name, "weight", weight)[1]
     dtype = x.dtype
@@ -1066,7 +1075,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     rows; ``A``: channels x states, ``D``, ``delta_bias``: channels, Float32.  D, z and delta_bias may be None.
     ``state``: Float32 slots x channels x states; it, ``offsets``, ``slots`` and ``initial`` are as in ``causal_conv``."""
     name = "selective_scan"
-    d = _dev(u)
+    d = _index(name, u)
     shape, states, groups, args = _scan_args(name, u, delta, A, B, C, D, z, delta_bias, d)
     rows, channels = shape
     count, at, flags = _sequences(name, offsets, initial, state, d)
@@ -1085,7 +1094,7 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, soft
     """One token per row: row r of ``u`` (rows x channels) continues state slot ``slots[r]`` (None: slot r), which
     is updated; the arguments are those of ``selective_scan``."""
     name = "selective_scan_step"
-    d = _dev(u)
+    d = _index(name, u)
     shape, states, groups, args = _scan_args(name, u, delta, A, B, C, D, z, delta_bias, d)
     rows, channels = shape
     if state is None:
