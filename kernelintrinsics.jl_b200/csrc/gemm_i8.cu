@@ -17,11 +17,17 @@
 //   warps 2-5  (2-9 from BN = 64) epilogue: TMEM -> registers -> scales -> C.
 // With few tiles the K blocks of a tile are split over the CTAs of a cluster; each CTA then leaves its
 // Int32 sums in its own shared memory and adds up and stores a share of the tile's columns, read from
-// every CTA of the cluster.  Rows that are not 16-byte aligned are loaded by warps 2-9 with plain loads.
+// every CTA of the cluster.  Rows that are not 16-byte aligned are loaded by warps 2-17 with plain loads.
 //
 // gemm_i8_pair_kernel, persistent CTA pairs on tiles of 256 channels x 256 tokens (cta_group::2): each CTA loads
 // 128 rows of either operand, each SM's TMEM holds two accumulators of its 128 channels x 256 tokens, so that the
 // epilogue of a tile runs beside the next tile's MMAs.
+//
+// Bounds and times (M x N x K, bf16 out; one B200): 8192 x 8192 x 4096 183-190 us, 2.9-3.0 P operations/s (tensor pipe 72 %
+// busy at 4096^3; the epilogue beside it: 236 us with four epilogue warps and scales from shuffles).  512 x 4096 x 4096 13.9 us.
+// 48 x 8192 x 4096 11.8 us and 1 x 4096 x 4096 6.4 us: the weight's bytes (5.3 and 2.6 us) and the latency of a launch, of the
+// first loads and of the join.  1111 x 4099 x 2057, rows at any byte: 61 us, bound by the integer instructions that
+// shift the loaded words into place.
 //
 // Every mbarrier wait is bounded, as in gemm_e4m3.cu.
 #include "ki/layer.cuh"
@@ -30,9 +36,6 @@
 
 namespace {
 
-#ifndef KI_I8_PAIRS
-#define KI_I8_PAIRS 60
-#endif
 constexpr int BM = 128, BK = 128;
 constexpr int LOADERS = 16;  // warps that load rows which TMA cannot, 16 each
 constexpr int THREADS_ROWS = 64 + 32 * LOADERS;
@@ -671,8 +674,11 @@ int launch(ki_ctx* ctx, GemmArgs& g, cudaStream_t s) {
     const long long tiles = (long long)g.ntiles * g.mtiles;
     if (tiles * MAX_SPLIT > 0x7fffffffll) return ki::set_error(ctx, KI_ERR_ARG, "gemm_i8: too many tiles");
     const int blocks = (g.k + BK - 1) / BK;
+    // Clusters of eight where there are few, or two CTAs fit an SM: sixteen clusters of eight CTAs that need an SM each do not
+    // run at once (128 x 2048 x 4096: 14.9 us in eight parts, 8.8 in four; 1 x 2048 x 4096: 5.8 and 6.3 us).
+    const int most = BN <= 32 || 16 * tiles <= ctx->sm_count ? MAX_SPLIT : 4;
     int split = 1;
-    while (split < MAX_SPLIT && 2 * split * tiles <= ctx->sm_count && 2 * split <= blocks) split *= 2;
+    while (split < most && 2 * split * tiles <= ctx->sm_count && 2 * split <= blocks) split *= 2;
     auto kern = gemm_i8_kernel<BN, O, TMA>;
     KI_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM_BYTES));
     cudaLaunchConfig_t cfg = {};
@@ -726,9 +732,10 @@ extern "C" int ki_gemm_i8(ki_ctx* ctx, const int8_t* d_A, size_t lda, const int8
     cudaStream_t s = ki::as_stream(stream);
     return ki::with_float_type(out_dtype, [&](auto t) {
         using O = decltype(t);
-        // pairs where their tiles fill the SMs
-        const long long tiles2 = (long long)((N + TILE2 - 1) / TILE2) * (long long)((M + TILE2 - 1) / TILE2);
-        if (tma && tiles2 >= KI_I8_PAIRS) return launch_pairs<O>(ctx, g, s);
+        // Pairs where the tiles of 128 x 128 would take more than one round: 768 x 4096 x 4096 17.0 us in pairs, 25.8 in
+        // two rounds of single tiles; 512 x 4096 x 4096 16.6 and 13.9 us in one round.
+        const long long tiles = (long long)((N + BM - 1) / BM) * (long long)((M + 127) / 128);
+        if (tma && M > 64 && tiles > ctx->sm_count) return launch_pairs<O>(ctx, g, s);
         if (M <= 16) return launch_tma<16, O>(ctx, g, tma, s);
         if (M <= 32) return launch_tma<32, O>(ctx, g, tma, s);
         if (M <= 64) return launch_tma<64, O>(ctx, g, tma, s);

@@ -7,15 +7,20 @@
 //
 // with g = d / (channels / groups); h is Float32 and starts from the sequence's slot or from zero.
 //
-// Bound: one exponential per token, channel and state (16 a clock and SM) at 16 states; the tokens'
-// bytes take a third of that time.  So every (d, n) pair has a lane slot of its own: LPC lanes share a
-// channel and each holds K states, the block walks the sequence in chunks of kChunk tokens, and the sums over
-// n are folded across the lanes LPC tokens at a time, which takes one shuffle per token and state pair.
+// Bound: one exponential per token, channel and state (16 a clock and SM) at 16 states, and the instructions around it;
+// the tokens' bytes take a third of that time.  The (channel, state) pairs are all the parallelism that one sequence has:
+// LPC lanes share a channel and hold K states each, and 128 such lanes walk the sequence in chunks of 32 tokens.  As many
+// helper threads bring the next chunk to shared memory as the lanes want it (steps through softplus, B and C side by
+// side) and finish the chunk before (sums over the lanes, D, gate, store), so that the lanes do nothing but the recurrence
+// and the two never wait for global memory.  At 8192 x 4096 x 16 bf16: 316 us (1240 us with one kind of thread, and the
+// sums folded by shuffles); the exponentials alone take 137 us.  Two warps per scheduler issue an instruction in 59 % of
+// the cycles there.  Tried without gain: loading and storing threads apart, two tokens per instruction instead of two
+// states, 64-token chunks, steps stored twice (shared-memory bandwidth: 82 -> 89 us at 2048 tokens), scalar arithmetic.
 #include "ki/layer.cuh"
 
 namespace {
 
-constexpr int kStepThreads = 256;
+constexpr int kStepThreads = 128;
 
 struct ScanArgs {
     const void* u;
@@ -475,7 +480,8 @@ __global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ?
     if (chunks > 0) finish(chunks - 1);
 }
 
-// One token per row: row r continues slot slots[r].  Bound: the states' bytes (one read and one write), so LPC lanes
+// One token per row: row r continues slot slots[r].  Bound: the states' bytes (one read and one write; 128 x 4096 x 16:
+// 18.2 us, 3.9 TB/s; one row at a time 26.5, two 20.5), so LPC lanes
 // share a channel with K states each (16 bytes and more per access) and take R rows at once: A is read once for them and
 // their states' loads are in flight together.  What is done once per row and channel (the step, the gate) is done
 // by lane r of the group for row r.
