@@ -341,8 +341,9 @@ int ki_gemm_e4m3_f32(ki_ctx* ctx, const uint8_t* d_A, const uint8_t* d_B, float*
  * padding, offsets are clamped to the rows, nothing outside the arrays is touched, and ki_ctx_check
  * reports KI_ERR_ARG. */
 /* Rows to int8: scale[r] = max|x[r, :]| * (1 / 127) and q = rint(x / scale[r]) (ties to even), the product
- * (with 1 / 127 as a Float32) and the quotient in IEEE Float32, q in [-127, 127].  scale 0 (a row of zeros, or cols = 0) gives q = 0; a row with a NaN
- * or an infinity has scale NaN or infinity (and q = 0 where x / scale is NaN or 0). */
+ * (with 1 / 127 as a Float32) and the quotient in IEEE Float32, q in [-127, 127].  scale 0 (a row of
+ * zeros, or cols = 0) gives q = 0; a row with a NaN or an infinity has scale NaN or infinity (and q = 0
+ * where x / scale is NaN or 0).  cols <= 2^31 - 4096. */
 int ki_quantize_rows(ki_ctx* ctx, int dtype, const void* d_x, size_t rows, size_t cols, size_t ld, int8_t* d_q,
                      size_t ldq, float* d_scale, void* stream);
 /* C[m, n] = (sum_k A[m, k] W[n, k]) * scale_a[m] * scale_w[n] + bias[n] with exact Int32 sums, on the

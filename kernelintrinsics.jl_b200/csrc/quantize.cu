@@ -205,7 +205,8 @@ extern "C" int ki_quantize_rows(ki_ctx* ctx, int dtype, const void* d_x, size_t 
     if (!es) return ki::set_error(ctx, KI_ERR_ARG, "quantize_rows: dtype must be KI_F32, KI_F16 or KI_BF16");
     if (rows == 0) return KI_OK;
     if (!d_scale || (cols > 0 && (!d_x || !d_q))) return ki::set_error(ctx, KI_ERR_ARG, "quantize_rows: null pointer");
-    if (cols > 0x7fffffffu) return ki::set_error(ctx, KI_ERR_ARG, "quantize_rows: too many columns");
+    // an int index may pass a row's end by four strides of 512 threads
+    if (cols > 0x7ffff000u) return ki::set_error(ctx, KI_ERR_ARG, "quantize_rows: too many columns");
     if (rows > 1 && (ld < cols || ldq < cols))
         return ki::set_error(ctx, KI_ERR_ARG, "quantize_rows: leading dimension smaller than cols");
     if (!ki::aligned(d_x, es) || !ki::aligned(d_scale, 4))

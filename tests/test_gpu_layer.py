@@ -658,6 +658,17 @@ def test_refusals_at_the_c_interface(KI, dev):
     assert ctypes.sizeof(ctypes.c_void_p) == 8
 
 
+def test_refuses_rows_at_the_end_of_32_bits(KI, dev):
+    """A thread's index passes the row's end by its stride before it stops, so rows end that much below 2^31."""
+    import torch
+
+    x = torch.zeros(8, device=dev)
+    for cols in (0x7ffff001, 0x7fffffff, 1 << 31, 1 << 40):
+        with pytest.raises(KI.KIArgumentError, match="too many columns"):
+            KI.context(0).call("ki_quantize_rows", 8, x.data_ptr() + 4, 1, cols, cols, x.data_ptr(), cols, x.data_ptr(),
+                               KI._stream_ptr(None, 0))
+
+
 def _layer(dev, seed=11, d=96, inner=160, states=16, rank=8):
     """Weights of one state-space layer: int8 projections with channel scales, convolution and scan parameters."""
     import torch
