@@ -339,7 +339,7 @@ int ki_gemm_e4m3_f32(ki_ctx* ctx, const uint8_t* d_A, const uint8_t* d_B, float*
  * the sequence's last row when the call is complete (an empty sequence: the state it started from).
  * Offsets and slots live on the device and are checked there: a slot number of `slots` or more is taken as
  * padding, offsets are clamped to the rows, nothing outside the arrays is touched, and ki_ctx_check
- * reports KI_ERR_ARG. */
+ * reports KI_ERR_ARG.  At most 2^31 - 4096 sequences.  No gradients: these are the served forms. */
 /* Rows to int8: scale[r] = max|x[r, :]| * (1 / 127) and q = rint(x / scale[r]) (ties to even), the product
  * (with 1 / 127 as a Float32) and the quotient in IEEE Float32, q in [-127, 127].  scale 0 (a row of
  * zeros, or cols = 0) gives q = 0; a row with a NaN or an infinity has scale NaN or infinity (and q = 0

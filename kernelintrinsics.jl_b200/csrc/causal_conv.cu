@@ -390,7 +390,7 @@ extern "C" int ki_causal_conv(ki_ctx* ctx, int dtype, const void* d_x, size_t ld
                               const uint8_t* d_initial, const int32_t* d_offsets, size_t seqs, void* d_y, size_t ldy,
                               size_t tokens, size_t channels, int width, int silu, void* stream) {
     KI_CHECK_CTX(ctx);
-    if (seqs > 0x7ffffffeu || slots > 0x7fffffffffffu)
+    if (seqs > ki::kMaxSequences || slots > 0x7fffffffffffu)
         return ki::set_error(ctx, KI_ERR_ARG, "causal_conv: too many sequences or slots");
     if (!d_offsets && seqs != 1) return ki::set_error(ctx, KI_ERR_ARG, "causal_conv: several sequences need offsets");
     ConvArgs a{d_x, ldx, d_w, d_bias, d_state, state_ld, d_y, ldy, 0, 0, silu != 0, false,
@@ -403,7 +403,7 @@ extern "C" int ki_causal_conv_step(ki_ctx* ctx, int dtype, const void* d_x, size
                                    const int32_t* d_slots, void* d_y, size_t ldy, size_t rows, size_t channels, int width,
                                    int silu, void* stream) {
     KI_CHECK_CTX(ctx);
-    if (rows > 0x7ffffffeu || slots > 0x7fffffffffffu)
+    if (rows > ki::kMaxSequences || slots > 0x7fffffffffffu)
         return ki::set_error(ctx, KI_ERR_ARG, "causal_conv_step: too many rows or slots");
     if (!d_state) return ki::set_error(ctx, KI_ERR_ARG, "causal_conv_step: null pointer");
     ConvArgs a{d_x, ldx, d_w, d_bias, d_state, state_ld, d_y, ldy, 0, 0, silu != 0, false,

@@ -127,6 +127,8 @@ __device__ __forceinline__ float softplus(float x) {
 // Sequence i holds tokens [offsets[i], offsets[i+1]) of the packed rows; without offsets there is one
 // sequence of all rows.  Offsets are read on the device, so they are clamped to the rows there are
 // and never trusted.
+constexpr size_t kMaxSequences = 0x7ffff000u;  // an int index may pass the last one by a block's threads
+
 struct Sequences {
     const int32_t* offsets;
     const int32_t* slots;    // state slot of each sequence; negative: the sequence is padding; null: slot i

@@ -684,7 +684,7 @@ extern "C" int ki_selective_scan(ki_ctx* ctx, int dtype, const void* d_u, size_t
                                  const uint8_t* d_initial, const int32_t* d_offsets, size_t seqs, void* d_y, size_t ldy,
                                  size_t tokens, size_t channels, size_t states, size_t groups, void* stream) {
     KI_CHECK_CTX(ctx);
-    if (seqs > 0x7ffffffeu || slots > 0x7fffffffffu)
+    if (seqs > ki::kMaxSequences || slots > 0x7fffffffffu)
         return ki::set_error(ctx, KI_ERR_ARG, "selective_scan: too many sequences or slots");
     if (!d_offsets && seqs != 1) return ki::set_error(ctx, KI_ERR_ARG, "selective_scan: several sequences need offsets");
     ScanArgs a{d_u, ldu, d_delta, ldd, d_A, d_B, ldb, d_C, ldc, d_D, d_z, ldz, d_delta_bias, d_state, state_ld, d_y, ldy,
@@ -699,7 +699,7 @@ extern "C" int ki_selective_scan_step(ki_ctx* ctx, int dtype, const void* d_u, s
                                       void* d_y, size_t ldy, size_t rows, size_t channels, size_t states, size_t groups,
                                       void* stream) {
     KI_CHECK_CTX(ctx);
-    if (rows > 0x7ffffffeu || slots > 0x7fffffffffu)
+    if (rows > ki::kMaxSequences || slots > 0x7fffffffffu)
         return ki::set_error(ctx, KI_ERR_ARG, "selective_scan_step: too many rows or slots");
     if (!d_state) return ki::set_error(ctx, KI_ERR_ARG, "selective_scan_step: null pointer");
     ScanArgs a{d_u, ldu, d_delta, ldd, d_A, d_B, ldb, d_C, ldc, d_D, d_z, ldz, d_delta_bias, d_state, state_ld, d_y, ldy,

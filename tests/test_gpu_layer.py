@@ -669,6 +669,24 @@ def test_refuses_rows_at_the_end_of_32_bits(KI, dev):
                                KI._stream_ptr(None, 0))
 
 
+def test_refuses_sequences_at_the_end_of_32_bits(KI, dev):
+    """A thread's index passes the last sequence by its stride before it stops, so their number ends that much below 2^31."""
+    import torch
+
+    x = torch.zeros(64, device=dev)
+    p, s, c = x.data_ptr(), KI._stream_ptr(None, 0), KI.context(0)
+    for n in (0x7ffff001, 0x7ffffffe, 1 << 31, 1 << 40):
+        for name, args in (
+                ("ki_causal_conv", (8, p, 4, p, None, None, 0, 0, None, None, p, n, p, 4, 4, 4, 4, 0, s)),
+                ("ki_causal_conv_step", (8, p, 4, p, None, p, 12, n, None, p, 4, n, 4, 4, 0, s)),
+                ("ki_selective_scan", (8, p, 4, p, 4, p, p, 4, p, 4, None, None, 0, None, 0, None, 0, 0, None, None, p, n, p,
+                                       4, 4, 4, 4, 1, s)),
+                ("ki_selective_scan_step", (8, p, 4, p, 4, p, p, 4, p, 4, None, None, 0, None, 0, p, 16, n, None, p, 4, n, 4, 4,
+                                            1, s))):
+            with pytest.raises(KI.KIArgumentError, match="too many"):
+                c.call(name, *args)
+
+
 def _layer(dev, seed=11, d=96, inner=160, states=16, rank=8):
     """Weights of one state-space layer: int8 projections with channel scales, convolution and scan parameters."""
     import torch
