@@ -17,7 +17,7 @@
 //   warps 2-5  (2-9 from BN = 64) epilogue: TMEM -> registers -> scales -> C.
 // With few tiles the K blocks of a tile are split over the CTAs of a cluster; each CTA then leaves its
 // Int32 sums in its own shared memory and adds up and stores a share of the tile's columns, read from
-// every CTA of the cluster.  Rows that are not 16-byte aligned are loaded by warps 2-17 with plain loads.
+// every CTA of the cluster.  Rows that are not 16-byte aligned are loaded by warps 2-17 (2-19 from BN = 160) with plain loads.
 //
 // gemm_i8_pair_kernel, persistent CTA pairs on tiles of 256 channels x 256 tokens (cta_group::2): each CTA loads
 // 128 rows of either operand, each SM's TMEM holds two accumulators of its 128 channels x 256 tokens, so that the
@@ -26,8 +26,8 @@
 // Bounds and times (M x N x K, bf16 out; one B200): 8192 x 8192 x 4096 183-190 us, 2.9-3.0 P operations/s (tensor pipe 72 %
 // busy at 4096^3; the epilogue beside it: 236 us with four epilogue warps and scales from shuffles).  512 x 4096 x 4096 13.9 us.
 // 48 x 8192 x 4096 11.8 us and 1 x 4096 x 4096 6.4 us: the weight's bytes (5.3 and 2.6 us) and the latency of a launch, of the
-// first loads and of the join.  1111 x 4099 x 2057, rows at any byte: 61 us, bound by the integer instructions that
-// shift the loaded words into place.
+// first loads and of the join.  1111 x 4099 x 2057, rows at any byte: 52.5 us, bound by the loads and the integer
+// instructions that shift the loaded words into place.
 //
 // Every mbarrier wait is bounded, as in gemm_e4m3.cu.
 #include "ki/layer.cuh"
@@ -37,8 +37,6 @@
 namespace {
 
 constexpr int BM = 128, BK = 128;
-constexpr int LOADERS = 16;  // warps that load rows which TMA cannot, 16 each
-constexpr int THREADS_ROWS = 64 + 32 * LOADERS;
 constexpr int W_BYTES = BM * BK;
 constexpr int MAX_SPLIT = 8;
 
@@ -52,15 +50,16 @@ struct Shape {
     static constexpr int X_BYTES = BN * BK;
     static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
     // two CTAs per SM, but one with a deeper ring for the widest tiles
-    static constexpr int STAGES = BN <= 16 ? 6 : BN <= 32 ? 5 : BN <= 64 ? 4 : 6;
+    static constexpr int STAGES = BN <= 16 ? 6 : BN <= 32 ? 5 : BN <= 64 ? 4 : BN <= 128 ? 6 : 5;
     static constexpr int SUM_BYTES = BM * BN * 4;  // a split's Int32 sums, over the ring
     static constexpr int RING_BYTES = STAGES * STAGE_BYTES > SUM_BYTES ? STAGES * STAGE_BYTES : SUM_BYTES;
     static constexpr int SA_COLS = BN < 32 ? 32 : BN;  // the tokens' scales, behind the barriers
     static constexpr int SMEM_BYTES = 1024 + RING_BYTES + 256 + 4 * SA_COLS;
-    static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
+    static constexpr int TMEM_COLS = BN < 32 ? 32 : BN <= 128 ? BN : 256;
     static constexpr int EPI_WARPS = BN < 64 ? 4 : 8;  // four per 32 TMEM lanes, or eight with half of the columns each
-    static constexpr int EPI_COLS = BN < 64 ? TMEM_COLS : BN / 2;
-    static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+    static constexpr int EPI_COLS = BN < 64 ? TMEM_COLS : (BN / 2 + 31) / 32 * 32;
+    static constexpr int LOADERS = BN <= 128 ? 16 : (BM + BN) / 16;  // warps that load rows which TMA cannot, 16 each
+    static constexpr int THREADS = 64 + 32 * (TMA ? EPI_WARPS : LOADERS);
 };
 
 struct GemmArgs {
@@ -182,7 +181,7 @@ __device__ __forceinline__ void store_columns(O* c, size_t ldc, const uint32_t (
 }
 
 template <int BN, class O, bool TMA>
-__global__ void __launch_bounds__(TMA ? Shape<BN, TMA>::THREADS : THREADS_ROWS, 1)
+__global__ void __launch_bounds__(Shape<BN, TMA>::THREADS, 1)
     gemm_i8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const GemmArgs g,
                    int split) {
     using S = Shape<BN, TMA>;
@@ -198,14 +197,14 @@ __global__ void __launch_bounds__(TMA ? Shape<BN, TMA>::THREADS : THREADS_ROWS, 
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int part = blockIdx.x % split, tile = blockIdx.x / split;
-    const int n0 = (tile % g.ntiles) * BM, m0 = (tile / g.ntiles) * BN;
+    const int n0 = (tile % g.ntiles) * BM, m0 = (tile / g.ntiles) * BN, end = min(g.m, m0 + BN);
     const int blocks = (g.k + BK - 1) / BK;
     const int kb0 = (int)((long long)blocks * part / split), kb1 = (int)((long long)blocks * (part + 1) / split);
 
-    for (int i = threadIdx.x; i < S::SA_COLS; i += blockDim.x) scales[i] = i < BN && m0 + i < g.m ? g.sa[m0 + i] : 0.0f;
+    for (int i = threadIdx.x; i < S::SA_COLS; i += blockDim.x) scales[i] = m0 + i < end ? g.sa[m0 + i] : 0.0f;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full0 + 8 * s), "r"(TMA ? 1 : LOADERS));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full0 + 8 * s), "r"(TMA ? 1 : S::LOADERS));
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty0 + 8 * s));
         }
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(tfull));
@@ -273,10 +272,10 @@ __global__ void __launch_bounds__(TMA ? Shape<BN, TMA>::THREADS : THREADS_ROWS, 
         }
     } else if (!TMA && warp >= 2) {
         // W's 128 rows, then A's BN, 16 to a warp
-        static_assert(BM + BN <= Rows::N * LOADERS && BN % Rows::N == 0, "16 rows per warp");
+        static_assert(BM + BN <= Rows::N * S::LOADERS && BN % Rows::N == 0, "16 rows per warp");
         const int r0 = Rows::N * (warp - 2);
         const bool some = r0 < BM + BN && kb0 < kb1, isw = r0 < BM;  // without an inner dimension there is nothing to read
-        const Rows rows(isw ? g.w : g.a, isw ? g.ldw : g.lda, isw ? n0 + r0 : m0 + r0 - BM, isw ? g.n : min(g.m, m0 + BN),
+        const Rows rows(isw ? g.w : g.a, isw ? g.ldw : g.lda, isw ? n0 + r0 : m0 + r0 - BM, isw ? g.n : end,
                         g.k, lane);
         int s = 0;
         uint32_t ph = 1;
@@ -325,7 +324,7 @@ __global__ void __launch_bounds__(TMA ? Shape<BN, TMA>::THREADS : THREADS_ROWS, 
         if (ok) {
 #pragma unroll 1
             for (int c0 = first; c0 < first + S::EPI_COLS; c0 += 32) {
-                if (m0 + c0 >= g.m) break;
+                if (m0 + c0 >= end) break;
                 uint32_t v[32];
                 if (kb1 > kb0) {
                     KI_TMEM_LD_X32(tmem + ((uint32_t)row << 16) + (uint32_t)c0, v);
@@ -337,7 +336,7 @@ __global__ void __launch_bounds__(TMA ? Shape<BN, TMA>::THREADS : THREADS_ROWS, 
                 if (split == 1) {
                     if (on)
                         store_columns(static_cast<O*>(g.c) + (size_t)(m0 + c0) * g.ldc + n, g.ldc, v, scales + c0, sw, bias,
-                                      g.m - m0 - c0);
+                                      end - m0 - c0);
                 } else {
 #pragma unroll
                     for (int j = 0; j < (BN < 32 ? BN : 32); ++j)
@@ -354,7 +353,7 @@ __global__ void __launch_bounds__(TMA ? Shape<BN, TMA>::THREADS : THREADS_ROWS, 
         if (!*abort) {
             // this CTA's share of the columns; a thread takes four neighbouring channels of one
             const int n = n0 + 4 * lane, live = min(max(g.n - n, 0), 4);
-            const int columns = min(BN, g.m - m0);
+            const int columns = end - m0;
             float sw[4], bias[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -688,7 +687,7 @@ int launch(ki_ctx* ctx, GemmArgs& g, cudaStream_t s) {
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(tiles * split));
-    cfg.blockDim = dim3(TMA ? S::THREADS : THREADS_ROWS);
+    cfg.blockDim = dim3(S::THREADS);
     cfg.dynamicSmemBytes = S::SMEM_BYTES;
     cfg.stream = s;
     cfg.attrs = attr;
@@ -739,6 +738,12 @@ extern "C" int ki_gemm_i8(ki_ctx* ctx, const int8_t* d_A, size_t lda, const int8
         if (M <= 16) return launch_tma<16, O>(ctx, g, tma, s);
         if (M <= 32) return launch_tma<32, O>(ctx, g, tma, s);
         if (M <= 64) return launch_tma<64, O>(ctx, g, tma, s);
+        // Rows that threads load: tiles of 160 tokens where that saves enough rounds.  A round of them takes a third
+        // longer (18 loading warps are five on a scheduler, not four; at K = 2057 26.7 and 20 us): 640 x 4099 x 2057 26.8 us in one
+        // round, 41.8 in two of 128 tokens; 1111 x 4099 x 2057 52.5 in two, 59.7 in three.
+        const long long wide = (long long)((N + BM - 1) / BM) * (long long)((M + 159) / 160);
+        auto rounds = [&](long long all) { return (all + ctx->sm_count - 1) / ctx->sm_count; };
+        if (!tma && 4 * rounds(wide) < 3 * rounds(tiles)) return launch<160, O, false>(ctx, g, s);
         return launch_tma<128, O>(ctx, g, tma, s);
     });
 }

@@ -171,6 +171,23 @@ def test_int8_gemm_strided(KI, dev, lead_a, lead_w, pad, M, N, K):
         assert (rest == 5.0).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(1111, 4099, 33), (640, 4099, 65), (513, 4099, 129), (740, 4099, 17), (768, 4100, 300),
+                                   (2100, 2049, 129), (769, 4099, 0)])
+def test_int8_gemm_tiles_of_other_widths(KI, dev, M, N, K):
+    """Rows that TMA cannot take, in more tiles of 128 x 128 than there are SMs; outputs at odd strides."""
+    import torch
+
+    a, w, sa, sw, bias = _operands(M + N + K, M, N, K, dev)
+    for dtype in (torch.float32, torch.bfloat16):
+        big = torch.full((M + 2, N + 5), 5.0, dtype=dtype, device=dev)
+        sc = sw * (max(K, 1) ** -0.5)
+        out = KI.int8_gemm(a, w, sa, sc, bias=bias, out=big[1:-1, 2:2 + N])
+        KI.context(0).check()
+        _check_product(out, a, w, sa, sc, bias, dtype)
+        big[1:-1, 2:2 + N] = 5.0
+        assert (big == 5.0).all()
+
+
 def test_int8_gemm_extremes(KI, dev):
     """The largest sums that are allowed, and no inner dimension at all."""
     import torch
