@@ -26,8 +26,8 @@
 // Bounds and times (M x N x K, bf16 out; one B200): 8192 x 8192 x 4096 183-190 us, 2.9-3.0 P operations/s (tensor pipe 72 %
 // busy at 4096^3; the epilogue beside it: 236 us with four epilogue warps and scales from shuffles).  512 x 4096 x 4096 13.9 us.
 // 48 x 8192 x 4096 11.8 us and 1 x 4096 x 4096 6.4 us: the weight's bytes (5.3 and 2.6 us) and the latency of a launch, of the
-// first loads and of the join.  1111 x 4099 x 2057, rows at any byte: 52.5 us, bound by the loads and the integer
-// instructions that shift the loaded words into place.
+// first loads and of the join.  1111 x 4099 x 2057, rows at any byte: 52.5 us, bound by the loading warps (the
+// integer pipe is 54 % busy with shifting the loaded words into place).
 //
 // Every mbarrier wait is bounded, as in gemm_e4m3.cu.
 #include "ki/layer.cuh"
