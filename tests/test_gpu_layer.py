@@ -889,3 +889,57 @@ def test_offsets_beyond_32_bits(KI, dev):
     sa = torch.ones(rows, device=dev)
     assert torch.equal(KI.int8_gemm(a, wt, sa, ws), KI.int8_gemm(a.contiguous(), wt, sa, ws))
     KI.context(0).check()
+
+
+# ---------------------------------------------------------------------------------------------
+# infinities and NaN
+# ---------------------------------------------------------------------------------------------
+def _as_defined(got, want, err, dtype):
+    """NaN and infinities where the definition has them, and elsewhere within the bound."""
+    got = ref.f64(got)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), np.argwhere(np.isnan(got) != np.isnan(want))[:5]
+    big = np.isinf(want)
+    assert np.array_equal(got[big], want[big])
+    fin = np.isfinite(want)
+    assert (np.abs(got[fin] - want[fin]) <= ref.stored(want[fin], err[fin], dtype)).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("soft", [False, True])
+@pytest.mark.parametrize("states,channels", [(1, 16), (5, 16), (13, 16), (16, 16), (17, 16), (24, 16), (33, 16), (100, 16),
+                                             (200, 16), (5, 2400), (13, 1200), (13, 2400), (24, 1200)])
+def test_selective_scan_of_infinities(KI, dev, dtype, soft, states, channels):
+    """An infinite input makes its channel infinite, not NaN, whatever the number of states, in the prompt's form and in
+    the single token's.  B, C and D are positive, so that no sum has infinities of both signs; decays stay far from zero
+    (at most 40 steps of 0.3), so that infinite states stay infinite."""
+    import torch
+
+    T = 40
+    g = _rng(states + channels)
+    c, state, _, _ = _scan_case(states, T, 1, channels, states, 1, dtype, dev, soft=soft)
+    c["B"], c["C"] = c["B"].abs() + 0.1, c["C"].abs() + 0.1
+    c["D"] = c["D"].abs()
+    c["A"] = -(torch.rand(channels, states, generator=g) + 0.5).to(dev)
+    if soft:
+        c["delta_bias"] = torch.full((channels,), -3.0, device=dev)
+        c["delta"] = c["delta"].clamp(-1, 1)
+        c["delta"][3, 6] = -1e4  # a step of zero
+    inf = float("inf")
+    c["u"][5, 0], c["u"][33, 1] = inf, -inf
+    c["delta"][9, 2], c["u"][9, 2] = inf, 0.75
+    c["z"][11, 3], c["z"][12, 4] = inf, -inf
+    c["u"][13, 5] = float("nan")
+    c["z"][14, 7] = float("nan")
+    with np.errstate(all="ignore"):
+        want, err, last, lasterr = ref.scan(*(ref.f64(c[k]) for k in ("u", "delta", "A", "B", "C", "D", "z")),
+                                            ref.f64(c["delta_bias"]) if soft else None, soft, [(0, T)], [ref.f64(state[0])])
+    assert np.isinf(want[5:, 0]).all() and np.isinf(want[33:, 1]).all() and np.isinf(want[9:, 2]).all()
+    held, token = state.clone(), state.clone()
+    _as_defined(KI.selective_scan(**c, state=held), want, err, c["u"].dtype)
+    _as_defined(held[0], last[0], lasterr[0], torch.float32)
+    rows = {k: v for k, v in c.items() if k in ("u", "delta", "B", "C", "z")}
+    fixed = {k: v for k, v in c.items() if k not in rows}
+    steps = [KI.selective_scan_step(**{k: v[t:t + 1] for k, v in rows.items()}, **fixed, state=token) for t in range(T)]
+    _as_defined(torch.cat(steps), want, err, c["u"].dtype)
+    _as_defined(token[0], last[0], lasterr[0], torch.float32)
+    KI.context(0).check()
