@@ -344,83 +344,132 @@ end
 # ---- operators of a state-space layer served in 8 bits -----------------------------------------
 # No counterpart in the reference.  Tokens are columns: a row-major tokens x channels matrix of the ABI is a
 # channels x tokens Julia matrix.  Elements are Float32, Float16 or BFloat16; offsets and slot numbers are device
-# arrays of 0-based Int32, as at the ABI.
+# arrays of 0-based Int32, as at the ABI.  The ABI takes addresses, so every array is checked here first: that it is a
+# device array of the current device, its element type, its size and how its elements lie.
 _ft(::Type{T}) where {T} = T === Float32 ? Cint(8) : T === Float16 ? Cint(10) : nameof(T) === :BFloat16 ? Cint(11) :
                            throw(ArgumentError("Float32, Float16 or BFloat16 elements, not $T"))
-function _opt(::Type{T}, x) where {T}
-    x === nothing && return CuPtr{T}(0)
-    eltype(x) === T || (T === UInt8 && eltype(x) === Bool) || throw(ArgumentError("elements of type $T, not $(eltype(x))"))
-    return CuPtr{T}(UInt(pointer(x)))
+_root(x) = parent(x) === x ? x : _root(parent(x))  # the array that a view is of
+function _ondevice(x, name)
+    x isa StridedCuArray || throw(ArgumentError("$name: device arrays (CuArray or strided views of one), not $(typeof(x))"))
+    CUDA.device(_root(x)) == CUDA.device() || throw(ArgumentError("$name: an array is on another device than the current one"))
+    return x
 end
-function _ld(x)  # elements from column to column
-    x === nothing && return 0
-    stride(x, 1) == 1 || throw(ArgumentError("columns must be contiguous"))
-    return stride(x, 2)
+_dense(x) = all(d -> size(x, d) == 1 || stride(x, d) == prod(size(x)[1:d-1]), 1:ndims(x))
+# The address of an array that may be left out: contiguous, of this element type (a flag may be Bool) and these sizes.
+function _opt(::Type{T}, x, dims::Dims, name) where {T}
+    x === nothing && return CuPtr{T}(0)
+    _ondevice(x, name)
+    eltype(x) === T || (T === UInt8 && eltype(x) === Bool) || throw(ArgumentError("$name: elements of type $T, not $(eltype(x))"))
+    size(x) == dims || throw(DimensionMismatch("$name: $dims elements, not $(size(x))"))
+    _dense(x) || throw(ArgumentError("$name: an array must be contiguous"))
+    return reinterpret(CuPtr{T}, pointer(x))
+end
+# The address of a matrix of these sizes whose columns are contiguous and follow each other at any distance, and that
+# distance in elements.
+function _cols(::Type{T}, x, dims::Dims{2}, name) where {T}
+    x === nothing && return CuPtr{T}(0), 0
+    _ondevice(x, name)
+    eltype(x) === T || throw(ArgumentError("$name: elements of type $T, not $(eltype(x))"))
+    size(x) == dims || throw(DimensionMismatch("$name: $dims elements, not $(size(x))"))
+    dims[1] <= 1 || stride(x, 1) == 1 || throw(ArgumentError("$name: columns must be contiguous"))
+    dims[2] <= 1 || stride(x, 2) >= dims[1] || throw(ArgumentError("$name: columns overlap"))
+    return pointer(x), dims[2] > 1 ? stride(x, 2) : dims[1]
 end
 
 "int8 columns of `x` and their scales: scale = max|x[:, t]| * (1/127), q = rint(x / scale), ties to even."
-function quantize_rows!(q::CuMatrix{Int8}, scale::CuVector{Float32}, x::StridedCuMatrix{T}) where {T}
-    size(q) == size(x) && length(scale) == size(x, 2) || throw(DimensionMismatch("quantize_rows!"))
-    _call(c -> ccall((:ki_quantize_rows, libki), Cint,
-                     (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, Csize_t, Csize_t, CuPtr{Int8}, Csize_t, CuPtr{Float32}, Ptr{Cvoid}),
-                     c, _ft(T), pointer(x), size(x, 2), size(x, 1), _ld(x), q, _ld(q), scale, _stream()))
+function quantize_rows!(q::StridedCuMatrix{Int8}, scale::CuVector{Float32}, x::StridedCuMatrix{T}) where {T}
+    name = "quantize_rows!"
+    K, n = size(x)
+    GC.@preserve q scale x begin
+        px, ldx = _cols(T, x, (K, n), name)
+        pq, ldq = _cols(Int8, q, (K, n), name)
+        ps = _opt(Float32, scale, (n,), name)
+        _call(c -> ccall((:ki_quantize_rows, libki), Cint,
+                         (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, Csize_t, Csize_t, CuPtr{Int8}, Csize_t, CuPtr{Float32}, Ptr{Cvoid}),
+                         c, _ft(T), px, n, K, ldx, pq, ldq, ps, _stream()))
+    end
     return q, scale
 end
 """C[n, m] = (sum_k A[k, m] W[k, n]) * sa[m] * sw[n] + bias[n] with exact Int32 sums: A (K x tokens), W (K x channels),
 C (channels x tokens)."""
 function int8_gemm!(C::StridedCuMatrix{T}, A::StridedCuMatrix{Int8}, W::StridedCuMatrix{Int8}, sa::CuVector{Float32},
                     sw::CuVector{Float32}; bias = nothing) where {T}
+    name = "int8_gemm!"
     K, M = size(A); N = size(W, 2)
-    size(W, 1) == K && size(C) == (N, M) && length(sa) == M && length(sw) == N || throw(DimensionMismatch("int8_gemm!"))
-    bias === nothing || length(bias) == N || throw(DimensionMismatch("int8_gemm!"))
-    _call(c -> ccall((:ki_gemm_i8, libki), Cint,
-                     (Ptr{Cvoid}, CuPtr{Int8}, Csize_t, CuPtr{Int8}, Csize_t, CuPtr{Float32}, CuPtr{Float32}, CuPtr{Float32},
-                      Cint, CuPtr{T}, Csize_t, Csize_t, Csize_t, Csize_t, Ptr{Cvoid}),
-                     c, pointer(A), _ld(A), pointer(W), _ld(W), sa, sw, _opt(Float32, bias), _ft(T), pointer(C),
-                     _ld(C), M, N, K, _stream()))
+    GC.@preserve C A W sa sw bias begin
+        pA, lda = _cols(Int8, A, (K, M), name)
+        pW, ldw = _cols(Int8, W, (K, N), name)
+        pC, ldc = _cols(T, C, (N, M), name)
+        psa = _opt(Float32, sa, (M,), name); psw = _opt(Float32, sw, (N,), name); pb = _opt(Float32, bias, (N,), name)
+        _call(c -> ccall((:ki_gemm_i8, libki), Cint,
+                         (Ptr{Cvoid}, CuPtr{Int8}, Csize_t, CuPtr{Int8}, Csize_t, CuPtr{Float32}, CuPtr{Float32}, CuPtr{Float32},
+                          Cint, CuPtr{T}, Csize_t, Csize_t, Csize_t, Csize_t, Ptr{Cvoid}),
+                         c, pA, lda, pW, ldw, psa, psw, pb, _ft(T), pC, ldc, M, N, K, _stream()))
+    end
     return C
 end
-# A cache of states: a x b x slots, and the sequences of packed tokens (columns).
-function _cache(state, a, b, slots, count, name)
-    state === nothing && return (0, 0)
-    size(state)[1:2] == (a, b) || throw(DimensionMismatch(name))
-    strides(state)[1:2] == (1, a) || throw(ArgumentError("$name: every slot of the state must be contiguous"))
-    slots === nothing ? size(state, 3) >= count : length(slots) == count || throw(DimensionMismatch(name))
-    return (stride(state, 3), size(state, 3))
+# A cache of states, a x b x slots, for `count` sequences: its address, the elements between its slots, their number.
+function _cache(::Type{T}, state, a, b, slots, count, name) where {T}
+    if state === nothing
+        slots === nothing || throw(ArgumentError("$name: slots without a state"))
+        return CuPtr{T}(0), 0, 0
+    end
+    _ondevice(state, name)
+    eltype(state) === T || throw(ArgumentError("$name: a state of $T, not $(eltype(state))"))
+    ndims(state) == 3 && size(state)[1:2] == (a, b) || throw(DimensionMismatch("$name: a state of $a x $b x slots, not $(size(state))"))
+    (a <= 1 || stride(state, 1) == 1) && (b <= 1 || stride(state, 2) == a) ||
+        throw(ArgumentError("$name: every slot of the state must be contiguous"))
+    n = size(state, 3)
+    ld = n > 1 ? stride(state, 3) : a * b
+    ld >= a * b || throw(ArgumentError("$name: slots of the state overlap"))
+    if slots === nothing && n < count
+        throw(DimensionMismatch("$name: $n state slots for $count sequences"))
+    end
+    return pointer(state), ld, n
 end
-_sequences(offsets) = offsets === nothing ? 1 : length(offsets) - 1
+function _sequences(offsets, name)
+    offsets === nothing && return 1
+    length(offsets) >= 1 || throw(DimensionMismatch("$name: offsets must hold one value more than there are sequences"))
+    return length(offsets) - 1
+end
 """Causal depthwise convolution of packed sequences: x, y (channels x tokens), w (width x channels), state
 (channels x (width-1) x slots), offsets (sequences + 1)."""
 function causal_conv!(y::StridedCuMatrix{T}, x::StridedCuMatrix{T}, w::CuMatrix{T}; bias = nothing, state = nothing,
                       offsets = nothing, slots = nothing, initial = nothing, silu::Bool = false) where {T}
-    D, n = size(x); W = size(w, 1); count = _sequences(offsets)
-    size(y) == size(x) && size(w, 2) == D || throw(DimensionMismatch("causal_conv!"))
-    sld, ns = _cache(state, D, W - 1, slots, count, "causal_conv!")
-    _call(c -> ccall((:ki_causal_conv, libki), Cint,
-                     (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, CuPtr{T}, CuPtr{T}, Csize_t, Csize_t, CuPtr{Int32},
-                      CuPtr{UInt8}, CuPtr{Int32}, Csize_t, CuPtr{T}, Csize_t, Csize_t, Csize_t, Cint, Cint, Ptr{Cvoid}),
-                     c, _ft(T), pointer(x), _ld(x), w, _opt(T, bias), _opt(T, state), sld, ns, _opt(Int32, slots),
-                     _opt(UInt8, initial), _opt(Int32, offsets), count, pointer(y), _ld(y), n, D, W, silu, _stream()))
+    name = "causal_conv!"
+    D, n = size(x); W = size(w, 1); count = _sequences(offsets, name)
+    GC.@preserve y x w bias state offsets slots initial begin
+        px, ldx = _cols(T, x, (D, n), name)
+        py, ldy = _cols(T, y, (D, n), name)
+        pw = _opt(T, w, (W, D), name); pb = _opt(T, bias, (D,), name)
+        ps, sld, ns = _cache(T, state, D, W - 1, slots, count, name)
+        pslots = _opt(Int32, slots, (count,), name); pinit = _opt(UInt8, initial, (count,), name)
+        poff = _opt(Int32, offsets, (count + 1,), name)
+        _call(c -> ccall((:ki_causal_conv, libki), Cint,
+                         (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, CuPtr{T}, CuPtr{T}, Csize_t, Csize_t, CuPtr{Int32},
+                          CuPtr{UInt8}, CuPtr{Int32}, Csize_t, CuPtr{T}, Csize_t, Csize_t, Csize_t, Cint, Cint, Ptr{Cvoid}),
+                         c, _ft(T), px, ldx, pw, pb, ps, sld, ns, pslots, pinit, poff, count, py, ldy, n, D, W, silu,
+                         _stream()))
+    end
     return y
 end
 "One token per column: column r continues slot `slots[r]` of the state."
 function causal_conv_step!(y::StridedCuMatrix{T}, x::StridedCuMatrix{T}, w::CuMatrix{T}, state::StridedCuArray{T,3}; bias = nothing,
                            slots = nothing, silu::Bool = false) where {T}
+    name = "causal_conv_step!"
     D, n = size(x); W = size(w, 1)
-    size(y) == size(x) && size(w, 2) == D || throw(DimensionMismatch("causal_conv_step!"))
-    sld, ns = _cache(state, D, W - 1, slots, n, "causal_conv_step!")
-    _call(c -> ccall((:ki_causal_conv_step, libki), Cint,
-                     (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, CuPtr{T}, CuPtr{T}, Csize_t, Csize_t, CuPtr{Int32},
-                      CuPtr{T}, Csize_t, Csize_t, Csize_t, Cint, Cint, Ptr{Cvoid}),
-                     c, _ft(T), pointer(x), _ld(x), w, _opt(T, bias), _opt(T, state), sld, ns, _opt(Int32, slots),
-                     pointer(y), _ld(y), n, D, W, silu, _stream()))
+    GC.@preserve y x w state bias slots begin
+        px, ldx = _cols(T, x, (D, n), name)
+        py, ldy = _cols(T, y, (D, n), name)
+        pw = _opt(T, w, (W, D), name); pb = _opt(T, bias, (D,), name)
+        ps, sld, ns = _cache(T, state, D, W - 1, slots, n, name)
+        pslots = _opt(Int32, slots, (n,), name)
+        _call(c -> ccall((:ki_causal_conv_step, libki), Cint,
+                         (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, CuPtr{T}, CuPtr{T}, Csize_t, Csize_t, CuPtr{Int32},
+                          CuPtr{T}, Csize_t, Csize_t, Csize_t, Cint, Cint, Ptr{Cvoid}),
+                         c, _ft(T), px, ldx, pw, pb, ps, sld, ns, pslots, py, ldy, n, D, W, silu, _stream()))
+    end
     return y
-end
-function _scan_sizes(u, delta, A, B, C, z, groups, y, name)
-    D, n = size(u); N = size(A, 1)
-    size(y) == size(u) && size(delta) == size(u) && size(A, 2) == D && size(B) == (groups * N, n) && size(C) == size(B) &&
-        (z === nothing || size(z) == size(u)) || throw(DimensionMismatch(name))
-    return D, n, N
 end
 """Selective scan of packed sequences: u, delta, z, y (channels x tokens), A (states x channels), B, C
 (groups*states x tokens), state (states x channels x slots, Float32)."""
@@ -428,33 +477,54 @@ function selective_scan!(y::StridedCuMatrix{T}, u::StridedCuMatrix{T}, delta::St
                          B::StridedCuMatrix{T}, C::StridedCuMatrix{T}; D = nothing, z = nothing, delta_bias = nothing,
                          softplus::Bool = false, state = nothing, offsets = nothing, slots = nothing, initial = nothing,
                          groups::Integer = 1) where {T}
-    d, n, N = _scan_sizes(u, delta, A, B, C, z, groups, y, "selective_scan!")
-    count = _sequences(offsets)
-    sld, ns = _cache(state, N, d, slots, count, "selective_scan!")
-    _call(c -> ccall((:ki_selective_scan, libki), Cint,
-                     (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{T},
-                      Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{Float32}, Cint, CuPtr{Float32}, Csize_t, Csize_t,
-                      CuPtr{Int32}, CuPtr{UInt8}, CuPtr{Int32}, Csize_t, CuPtr{T}, Csize_t, Csize_t, Csize_t, Csize_t,
-                      Csize_t, Ptr{Cvoid}),
-                     c, _ft(T), pointer(u), _ld(u), pointer(delta), _ld(delta), A, pointer(B), _ld(B),
-                     pointer(C), _ld(C), _opt(Float32, D), _opt(T, z), _ld(z), _opt(Float32, delta_bias), softplus,
-                     _opt(Float32, state), sld, ns, _opt(Int32, slots), _opt(UInt8, initial), _opt(Int32, offsets), count,
-                     pointer(y), _ld(y), n, d, N, groups, _stream()))
+    name = "selective_scan!"
+    d, n = size(u); N = size(A, 1); count = _sequences(offsets, name)
+    GC.@preserve y u delta A B C D z delta_bias state offsets slots initial begin
+        pu, ldu = _cols(T, u, (d, n), name)
+        pd, ldd = _cols(T, delta, (d, n), name)
+        py, ldy = _cols(T, y, (d, n), name)
+        pz, ldz = _cols(T, z, (d, n), name)
+        pB, ldb = _cols(T, B, (groups * N, n), name)
+        pC, ldc = _cols(T, C, (groups * N, n), name)
+        pA = _opt(Float32, A, (N, d), name)
+        pD = _opt(Float32, D, (d,), name); pbias = _opt(Float32, delta_bias, (d,), name)
+        ps, sld, ns = _cache(Float32, state, N, d, slots, count, name)
+        pslots = _opt(Int32, slots, (count,), name); pinit = _opt(UInt8, initial, (count,), name)
+        poff = _opt(Int32, offsets, (count + 1,), name)
+        _call(c -> ccall((:ki_selective_scan, libki), Cint,
+                         (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{T},
+                          Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{Float32}, Cint, CuPtr{Float32}, Csize_t, Csize_t,
+                          CuPtr{Int32}, CuPtr{UInt8}, CuPtr{Int32}, Csize_t, CuPtr{T}, Csize_t, Csize_t, Csize_t, Csize_t,
+                          Csize_t, Ptr{Cvoid}),
+                         c, _ft(T), pu, ldu, pd, ldd, pA, pB, ldb, pC, ldc, pD, pz, ldz, pbias, softplus, ps, sld, ns,
+                         pslots, pinit, poff, count, py, ldy, n, d, N, groups, _stream()))
+    end
     return y
 end
 "One token per column: column r continues slot `slots[r]` of the state."
 function selective_scan_step!(y::StridedCuMatrix{T}, u::StridedCuMatrix{T}, delta::StridedCuMatrix{T}, A::CuMatrix{Float32},
                               B::StridedCuMatrix{T}, C::StridedCuMatrix{T}, state::StridedCuArray{Float32,3}; D = nothing, z = nothing,
                               delta_bias = nothing, softplus::Bool = false, slots = nothing, groups::Integer = 1) where {T}
-    d, n, N = _scan_sizes(u, delta, A, B, C, z, groups, y, "selective_scan_step!")
-    sld, ns = _cache(state, N, d, slots, n, "selective_scan_step!")
-    _call(c -> ccall((:ki_selective_scan_step, libki), Cint,
-                     (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{T},
-                      Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{Float32}, Cint, CuPtr{Float32}, Csize_t, Csize_t,
-                      CuPtr{Int32}, CuPtr{T}, Csize_t, Csize_t, Csize_t, Csize_t, Csize_t, Ptr{Cvoid}),
-                     c, _ft(T), pointer(u), _ld(u), pointer(delta), _ld(delta), A, pointer(B), _ld(B),
-                     pointer(C), _ld(C), _opt(Float32, D), _opt(T, z), _ld(z), _opt(Float32, delta_bias), softplus,
-                     _opt(Float32, state), sld, ns, _opt(Int32, slots), pointer(y), _ld(y), n, d, N, groups, _stream()))
+    name = "selective_scan_step!"
+    d, n = size(u); N = size(A, 1)
+    GC.@preserve y u delta A B C state D z delta_bias slots begin
+        pu, ldu = _cols(T, u, (d, n), name)
+        pd, ldd = _cols(T, delta, (d, n), name)
+        py, ldy = _cols(T, y, (d, n), name)
+        pz, ldz = _cols(T, z, (d, n), name)
+        pB, ldb = _cols(T, B, (groups * N, n), name)
+        pC, ldc = _cols(T, C, (groups * N, n), name)
+        pA = _opt(Float32, A, (N, d), name)
+        pD = _opt(Float32, D, (d,), name); pbias = _opt(Float32, delta_bias, (d,), name)
+        ps, sld, ns = _cache(Float32, state, N, d, slots, n, name)
+        pslots = _opt(Int32, slots, (n,), name)
+        _call(c -> ccall((:ki_selective_scan_step, libki), Cint,
+                         (Ptr{Cvoid}, Cint, CuPtr{T}, Csize_t, CuPtr{T}, Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{T},
+                          Csize_t, CuPtr{Float32}, CuPtr{T}, Csize_t, CuPtr{Float32}, Cint, CuPtr{Float32}, Csize_t, Csize_t,
+                          CuPtr{Int32}, CuPtr{T}, Csize_t, Csize_t, Csize_t, Csize_t, Csize_t, Ptr{Cvoid}),
+                         c, _ft(T), pu, ldu, pd, ldd, pA, pB, ldb, pC, ldc, pD, pz, ldz, pbias, softplus, ps, sld, ns,
+                         pslots, py, ldy, n, d, N, groups, _stream()))
+    end
     return y
 end
 

@@ -127,3 +127,48 @@ def test_library_path_points_at_the_in_tree_build():
     src = JL.read_text()
     assert 'joinpath(@__DIR__, "..", "lib", "libki_b200.so")' in src
     assert (JL.parent / ".." / "lib").resolve() == (PKG / "lib").resolve()
+
+
+def _layer_functions() -> dict:
+    """Name -> source of each function of the state-space layer's operators, comments removed."""
+    src = JL.read_text()
+    part = src[src.index("# ---- operators of a state-space layer"):src.index("# ---- several GPUs")]
+    part = re.sub(r"#[^\n]*", "", part)
+    return {m.group(1): m.group(0) for m in re.finditer(r"^function ([\w!]+)\(.*?^end$", part, flags=re.M | re.S)}
+
+
+LAYER = ("quantize_rows!", "int8_gemm!", "causal_conv!", "causal_conv_step!", "selective_scan!", "selective_scan_step!")
+
+
+def test_layer_operators_give_only_checked_addresses():
+    """An address at the ABI comes from a function that compares device, type, size and strides with what is asked for, and
+    every array stays alive across the call."""
+    fns = _layer_functions()
+    for checker, needed in (("_opt", ("_ondevice(", "eltype(x) === T", "size(x) == dims", "_dense(x)")),
+                            ("_cols", ("_ondevice(", "eltype(x) === T", "size(x) == dims", "stride(x, 1) == 1", "stride(x, 2) >=")),
+                            ("_cache", ("_ondevice(", "eltype(state) === T", "size(state)[1:2] ==", "stride(state, 2) == a"))):
+        for text in needed:
+            assert text in fns[checker], (checker, text)
+    assert "isa StridedCuArray" in fns["_ondevice"] and "CUDA.device()" in fns["_ondevice"]
+    for name in LAYER:
+        src = fns[name]
+        addresses = set()
+        for m in re.finditer(r"([\w, ]+?) = (_opt|_cols|_cache)(\()", src):
+            args = _split_top(src[m.end() - 1:][1:_balanced(src[m.end() - 1:], 0) - 1])
+            assert len(args) == {"_opt": 4, "_cols": 4, "_cache": 7}[m.group(2)], (name, m.group(0))
+            assert m.group(2) == "_cache" or args[2].startswith("("), (name, args)  # the sizes are stated
+            addresses.add((m.group(1).split(",")[0].strip(), args[1]))
+        assert "pointer(" not in src, name
+        kept = re.search(r"GC\.@preserve ([^\n]*) begin", src).group(1).split()
+        assert {array for _, array in addresses} <= set(kept), name
+        call = src[src.index("ccall("):]
+        types, args = [c for c in julia_ccalls() if c[0] == re.search(r":(ki_\w+)", call).group(1)][0][2:]
+        for t, a in zip(types, args):
+            if t.startswith("CuPtr"):
+                assert a in {p for p, _ in addresses}, (name, a)
+
+
+def test_layer_operators_throw_where_they_mean_to():
+    """`a ? b : c || throw(...)` throws on c alone."""
+    for name, src in _layer_functions().items():
+        assert not re.search(r" \? [^\n]* : [^\n]*\|\| *throw", src), name
