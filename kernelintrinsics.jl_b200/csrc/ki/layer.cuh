@@ -70,6 +70,12 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // x * sigmoid(x); -inf gives NaN as the formula does.
 __device__ __forceinline__ float silu(float x) { return x * rcp_fast(1.0f + exp2_fast(-kLog2e * x)); }
 
+// x log2(e), finite wherever x is: a step of zero then leaves a state as it is however large the magnitude of A (0 * inf would be NaN).
+__device__ __forceinline__ float times_log2e(float x) {
+    const float y = x * kLog2e, top = 3.402823466e38f;
+    return fabsf(x) <= top ? fminf(fmaxf(y, -top), top) : y;
+}
+
 // Two Float32 in one register pair; one instruction works on both.
 using f32x2 = unsigned long long;
 __device__ __forceinline__ f32x2 pair(float lo, float hi) {

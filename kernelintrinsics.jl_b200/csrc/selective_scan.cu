@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ?
         for (int k = 0; k < K; ++k) {
             const bool on = dl < width && ln * K + k < a.states;
             const size_t at = (size_t)(d0 + dl) * a.states + ln * K + k;
-            A[k] = on ? a.A[at] * ki::kLog2e : 0.0f;
+            A[k] = on ? ki::times_log2e(a.A[at]) : 0.0f;
             h[k] = on && keep ? st[at] : 0.0f;
         }
 #pragma unroll
@@ -532,16 +532,17 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const ScanArgs 
         if (a.delta_bias) s += a.delta_bias[d];
         if (a.soft) s = ki::softplus(s);
     }
+    const float s2 = ki::times_log2e(s);
     float y = 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const float sr = __shfl_sync(0xffffffffu, s, r, LPC);
+        const float sr = __shfl_sync(0xffffffffu, s2, r, LPC);
         const float su = __shfl_sync(0xffffffffu, s * u, r, LPC);
         float p = 0.0f;
         if (slot[r] >= 0 && live) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const float v = fmaf(ki::exp2_fast(sr * (A.get(k) * ki::kLog2e)), h[r].get(k), su * ki::to_f32(b[r].get(k)));
+                const float v = fmaf(ki::exp2_fast(sr * A.get(k)), h[r].get(k), su * ki::to_f32(b[r].get(k)));
                 h[r].w[k] = __float_as_uint(v);
                 if (k < n) p = fmaf(ki::to_f32(c[r].get(k)), v, p);
             }

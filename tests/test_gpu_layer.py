@@ -943,3 +943,36 @@ def test_selective_scan_of_infinities(KI, dev, dtype, soft, states, channels):
     _as_defined(torch.cat(steps), want, err, c["u"].dtype)
     _as_defined(token[0], last[0], lasterr[0], torch.float32)
     KI.context(0).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("states,channels", [(16, 24), (13, 24), (16, 2400), (64, 24)])
+def test_selective_scan_of_the_lowest_decays(KI, dev, dtype, states, channels):
+    """A of the lowest value forgets a state at any step, but a step of zero leaves it as it is; so does minus infinity
+    where no step is zero."""
+    import torch
+
+    T = 37
+    c, state, _, _ = _scan_case(states, T, 1, channels, states, 1, dtype, dev, soft=False)
+    c["delta"] = c["delta"] + 0.01
+    low = dict(c, A=c["A"].clone())
+    low["A"][:, 0] = -1e30
+    low["A"][:, -1] = -float("inf")
+    same = dict(c, A=low["A"].clamp(min=-1e30))
+    held = [state.clone(), state.clone()]
+    assert torch.equal(KI.selective_scan(**low, state=held[0]), KI.selective_scan(**same, state=held[1]))
+    assert torch.equal(*held)
+    c["A"][:, 0] = torch.finfo(torch.float32).min
+    c["A"][1, -1] = torch.finfo(torch.float32).min
+    c["delta"][::3] = 0
+    want, err, last, lasterr = ref.scan(*(ref.f64(c[k]) for k in ("u", "delta", "A", "B", "C", "D", "z")), None, False,
+                                        [(0, T)], [ref.f64(state[0])])
+    held, token = state.clone(), state.clone()
+    _within(KI.selective_scan(**c, state=held), want, err, c["u"].dtype)
+    _within(held[0], last[0], lasterr[0], torch.float32)
+    rows = {k: v for k, v in c.items() if k in ("u", "delta", "B", "C", "z")}
+    fixed = {k: v for k, v in c.items() if k not in rows}
+    steps = [KI.selective_scan_step(**{k: v[t:t + 1] for k, v in rows.items()}, **fixed, state=token) for t in range(T)]
+    _within(torch.cat(steps), want, err, c["u"].dtype)
+    _within(token[0], last[0], lasterr[0], torch.float32)
+    KI.context(0).check()
