@@ -193,9 +193,8 @@ _ctx_by_key: dict = {}
 
 def context(device: Optional[int] = None) -> Context:
     """The calling thread's context on ``device`` (default: torch's current device)."""
-    torch = _torch()
     if device is None:
-        device = torch.cuda.current_device()
+        device = _torch().cuda.current_device()
     key = (threading.get_ident(), int(device))
     c = _ctx_by_key.get(key)  # only this thread makes the entry
     if c is None:
@@ -782,6 +781,8 @@ def fp8_gemm(A, B, C=None, scale_a: float = 1.0, scale_b: float = 1.0, stream=No
 # ---------------------------------------------------------------------------------------------
 # operators of a state-space layer served in 8 bits.  Single-token calls take less time on the GPU
 # than in Python, so these checks read each tensor's properties once and build messages only to raise.
+# These are served forms without gradients: a tensor that requires one is refused while torch records gradients,
+# rather than its gradient lost.
 # ---------------------------------------------------------------------------------------------
 _float_codes: dict = {}
 
@@ -814,6 +815,11 @@ def _refuse(name: str, what: str, t, shape: tuple, dtype, d: int, how: str):
     raise _bad(f"{name}: {what} must {how}")
 
 
+def _no_gradient(name: str, what: str):
+    if _torch().is_grad_enabled():
+        raise _bad(f"{name}: {what} requires a gradient, and this operator has none: detach it or call under torch.no_grad()")
+
+
 def _rows(name: str, what: str, t, shape: tuple, dtype, d: int) -> int:
     """The row stride of a 2-D ``t`` of this shape and type on device ``d`` whose rows are contiguous."""
     if t.dtype is not dtype or t.shape != shape or t.get_device() != d:
@@ -822,6 +828,8 @@ def _rows(name: str, what: str, t, shape: tuple, dtype, d: int) -> int:
     ld, inner = t.stride()
     if (inner != 1 and cols > 1) or (ld < cols and rows > 1):
         _refuse(name, what, t, shape, dtype, d, "have contiguous rows that do not overlap")
+    if t.requires_grad:
+        _no_gradient(name, what)
     return ld if rows > 1 else cols
 
 
@@ -831,6 +839,8 @@ def _flat(name: str, what: str, t, shape: tuple, dtype, d: int):
         return None
     if t.dtype is not dtype or t.shape != shape or t.get_device() != d or not t.is_contiguous():
         _refuse(name, what, t, shape, dtype, d, "be contiguous")
+    if t.requires_grad:
+        _no_gradient(name, what)
     return t.data_ptr()
 
 
@@ -850,12 +860,18 @@ def _like(x, dtype, stream):
         return _torch().empty_like(x, dtype=dtype)
 
 
+_current_raw_stream = None
+
+
 def _raw_stream(stream, d: int) -> int:
+    global _current_raw_stream
     if stream is not None:
         if stream.device.index != d:
             raise _bad(f"stream of cuda:{stream.device.index} for tensors on cuda:{d}")
         return stream.cuda_stream
-    return _torch()._C._cuda_getCurrentRawStream(d)
+    if _current_raw_stream is None:
+        _current_raw_stream = _torch()._C._cuda_getCurrentRawStream
+    return _current_raw_stream(d)
 
 
 def _state(name: str, state, first: int, second: int, dtype, d: int, slots, count: int):
@@ -866,6 +882,8 @@ def _state(name: str, state, first: int, second: int, dtype, d: int, slots, coun
         return None, 0, 0, None
     if state.dtype is not dtype or state.dim() != 3 or state.shape[1:] != (first, second) or state.get_device() != d:
         raise _bad(f"{name}: state must be {dtype} [slots, {first}, {second}] on cuda:{d}")
+    if state.requires_grad:
+        _no_gradient(name, "state")
     n, held = state.shape[0], first * second
     ld = held
     if not state.is_contiguous():
@@ -919,7 +937,7 @@ def _matrix(name: str, what: str, t) -> tuple:
 def quantize_rows(x, out=None, scale=None, stream=None):
     """int8 rows with one scale each: scale[r] = max|x[r]| * (1 / 127), out[r] = rint(x[r] / scale[r]) (ties
     to even, all in Float32), for a 2-D Float32, Float16 or BFloat16 ``x`` with contiguous rows.
-    A row of zeros gives zeros and scale 0; a NaN or an infinity stays in the row's scale.
+    A row of zeros gives zeros and scale 0; a NaN or an infinity stays in the row's scale.  No gradient.
     Returns (out, scale): int8 of x's shape, Float32 per row."""
     torch = _torch()
     name = "quantize_rows"
@@ -944,7 +962,7 @@ def quantize_rows(x, out=None, scale=None, stream=None):
 def int8_gemm(A, W, scale_a, scale_w, bias=None, out=None, dtype=None, stream=None):
     """out[m, n] = (sum_k A[m, k] W[n, k]) * scale_a[m] * scale_w[n] + bias[n] with exact Int32 sums on the
     tensor cores: int8 tokens ``A`` (M x K) and weights ``W`` (N x K) with contiguous rows, Float32 scales per
-    token and per channel, Float32 ``bias`` or None.  ``out`` has ``dtype`` (bfloat16 unless given)."""
+    token and per channel, Float32 ``bias`` or None.  ``out`` has ``dtype`` (bfloat16 unless given).  No gradient."""
     torch = _torch()
     name = "int8_gemm"
     d = _index(name, A)
@@ -980,7 +998,7 @@ def causal_conv(x, weight, bias=None, state=None, offsets=None, slots=None, init
     numbers mark padding that is skipped, and no slot is named twice.  ``initial`` (bool or uint8): False
     starts the sequence from zeros.  Without a state every sequence starts from zeros.  Rows of no sequence
     are not written (a new output holds anything there).  A bad offset or slot number is reported by
-    ``Context.check``."""
+    ``Context.check``.  No gradient."""
     name = "causal_conv"
     d = _index(name, x)
     tokens, channels = shape = _matrix(name, "x", x)
@@ -1040,6 +1058,8 @@ def _per_state(name: str, what: str, t, rows: int, states: int, dtype, d: int) -
     ld, mid, inner = t.stride()
     if (inner != 1 and states > 1) or (mid != states and groups > 1) or (ld < groups * states and rows > 1):
         _refuse(name, what, t, shape, dtype, d, "have contiguous rows that do not overlap")
+    if t.requires_grad:
+        _no_gradient(name, what)
     return (ld if rows > 1 else groups * states), groups
 
 
@@ -1073,7 +1093,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     ``u``, ``delta``, ``z``: tokens x channels; ``B``, ``C``: tokens x states, or tokens x groups x states (channel d
     belongs to group d // (channels / groups)), all of one type (Float32, Float16, BFloat16) with contiguous
     rows; ``A``: channels x states, ``D``, ``delta_bias``: channels, Float32.  D, z and delta_bias may be None.
-    ``state``: Float32 slots x channels x states; it, ``offsets``, ``slots`` and ``initial`` are as in ``causal_conv``."""
+    ``state``: Float32 slots x channels x states; it, ``offsets``, ``slots`` and ``initial`` are as in ``causal_conv``.
+    No gradient."""
     name = "selective_scan"
     d = _index(name, u)
     shape, states, groups, args = _scan_args(name, u, delta, A, B, C, D, z, delta_bias, d)

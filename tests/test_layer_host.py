@@ -141,3 +141,20 @@ def test_reference_product():
     y, err = ref.product(a, w, np.ones(3), np.full(5, 0.5), np.arange(5.0))
     want = (torch.from_numpy(a).double() @ torch.from_numpy(w).double().t() * 0.5 + torch.arange(5.0)).numpy()
     assert np.array_equal(y, want) and (err >= 0).all()
+
+
+def test_tensors_that_require_gradients_are_refused():
+    """The operators give no gradients, so a tensor that requires one is refused where torch would record it."""
+    t = torch.zeros(6, 32, requires_grad=True)
+    state = torch.zeros(5, 4, 8, requires_grad=True)
+    grouped = t.unflatten(1, (2, 16))
+    calls = ((KI._rows, "f", "x", t, (6, 32), torch.float32, CPU), (KI._flat, "f", "x", t, (6, 32), torch.float32, CPU),
+             (KI._state, "f", state, 4, 8, torch.float32, CPU, None, 5),
+             (KI._per_state, "f", "B", grouped, 6, 16, torch.float32, CPU),
+             (KI._per_state, "f", "B", t, 6, 32, torch.float32, CPU))
+    for call, *args in calls:
+        with pytest.raises(KI.KIArgumentError, match="gradient"):
+            call(*args)
+        with torch.no_grad():
+            call(*args)
+        call(*(a.detach() if isinstance(a, torch.Tensor) else a for a in args))
