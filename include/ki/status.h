@@ -12,7 +12,7 @@
 enum : uint32_t {
     KI_DEV_TIMEOUT = 1u,   /* a bounded wait ran out */
     KI_DEV_BAD_STATE = 2u, /* a kernel saw an impossible value (e.g. a corrupt tile flag) */
-    KI_DEV_BAD_INDEX = 4u  /* an offset or a slot number in device memory was out of range */
+    KI_DEV_BAD_INDEX = 4u  /* an offset or a slot number in device memory was out of range (and was skipped) */
 };
 
 #endif /* KI_STATUS_H */

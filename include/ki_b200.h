@@ -88,8 +88,9 @@ int ki_ctx_destroy(ki_ctx* ctx);
  * had no context to hold it (a communicator whose set-up failed). */
 const char* ki_last_error_string(const ki_ctx* ctx);
 /* Synchronises `stream`, returns KI_ERR_TIMEOUT if any device-side wait of this context ran out
- * since the last check, KI_ERR_ARG if a kernel met an offset or a slot number (read on the device) that
- * was out of range (and clears both latches), KI_ERR_CUDA on an asynchronous CUDA error. */
+ * since the last check, else KI_ERR_CUDA if a kernel saw an inconsistent state (or on an asynchronous CUDA
+ * error), else KI_ERR_ARG if one met an offset or a slot number (read on the device) that was out of range;
+ * clears what was latched. */
 int ki_ctx_check(ki_ctx* ctx, void* stream);
 /* Limit of every device-side wait of this context (default 2 s). */
 int ki_ctx_set_wait_timeout_ns(ki_ctx* ctx, uint64_t ns);

@@ -122,11 +122,8 @@ int ki_ctx_check(ki_ctx* ctx, void* stream) {
     KI_CUDA(ctx, cudaMemcpy(&st, ctx->d_status, sizeof(st), cudaMemcpyDeviceToHost));
     if (st) {
         KI_CUDA(ctx, cudaMemset(ctx->d_status, 0, sizeof(uint32_t)));
-        if (st & KI_DEV_TIMEOUT)
-            return ki::set_error(ctx, KI_ERR_TIMEOUT, "a device-side wait ran out (status 0x%x)", st);
-        if (st & KI_DEV_BAD_INDEX)
-            return ki::set_error(ctx, KI_ERR_ARG, "an offset or a slot number in device memory was out of range (status 0x%x)", st);
-        return ki::set_error(ctx, KI_ERR_CUDA, "device reported an inconsistent state (status 0x%x)", st);
+        const ki::Latched l = ki::latched(st);
+        return ki::set_error(ctx, l.status, "%s (status 0x%x)", l.what, st);
     }
     return KI_OK;
 }

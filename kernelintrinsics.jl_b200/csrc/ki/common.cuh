@@ -80,6 +80,18 @@ inline int cuda_error(ki_ctx* ctx, cudaError_t e, const char* what) {
     return set_error(ctx, KI_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
 }
 
+// What a status word that is not zero is reported as: the gravest of the bits that are set.  A wait that ran out or an
+// impossible value says that results cannot be trusted; a bad index was skipped.
+struct Latched {
+    int status;
+    const char* what;
+};
+inline Latched latched(uint32_t bits) {
+    if (bits & KI_DEV_TIMEOUT) return {KI_ERR_TIMEOUT, "a device-side wait ran out"};
+    if (bits & ~(uint32_t)KI_DEV_BAD_INDEX) return {KI_ERR_CUDA, "device reported an inconsistent state"};
+    return {KI_ERR_ARG, "an offset or a slot number in device memory was out of range"};
+}
+
 // Make ctx->device current for the duration of a call.
 struct DeviceGuard {
     int prev = -1;

@@ -178,7 +178,8 @@ class Context:
             self._raise(st, name)
 
     def check(self, stream=None) -> None:
-        """Synchronise ``stream`` and raise if a bounded device-side wait of this context ran out."""
+        """Synchronise ``stream`` and raise if a bounded device-side wait of this context ran out, or a kernel met an offset
+        or a slot number in device memory that was out of range."""
         st = self.lib.ki_ctx_check(self.handle, _stream_ptr(stream, self.device))
         if st != _abi.KI_OK:
             self._raise(st, "ki_ctx_check")

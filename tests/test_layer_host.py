@@ -158,3 +158,19 @@ def test_tensors_that_require_gradients_are_refused():
         with torch.no_grad():
             call(*args)
         call(*(a.detach() if isinstance(a, torch.Tensor) else a for a in args))
+
+
+def test_the_gravest_latched_bit_is_reported(tmp_path):
+    """A status word with a bad index and an inconsistent state says inconsistent state; a wait that ran out comes first."""
+    import subprocess
+
+    from conftest import PKG
+
+    src = tmp_path / "latched.cpp"
+    src.write_text('#include <cstdio>\n#include "ki/common.cuh"\n'
+                   'int main() { for (unsigned b = 1; b < 8; ++b) std::printf("%d ", ki::latched(b).status); }\n')
+    exe = tmp_path / "latched"
+    subprocess.run(["g++", "-std=c++17", f"-I{PKG / 'csrc'}", "-I/usr/local/cuda/include", str(src), "-o", str(exe)], check=True)
+    # KI_DEV_TIMEOUT 1 -> KI_ERR_TIMEOUT 3, KI_DEV_BAD_STATE 2 -> KI_ERR_CUDA 2, KI_DEV_BAD_INDEX 4 -> KI_ERR_ARG 1
+    got = subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()
+    assert got == ["3", "2", "3", "1", "3", "2", "3"]
