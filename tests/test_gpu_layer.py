@@ -976,3 +976,130 @@ def test_selective_scan_of_the_lowest_decays(KI, dev, dtype, states, channels):
     _within(torch.cat(steps), want, err, c["u"].dtype)
     _within(token[0], last[0], lasterr[0], torch.float32)
     KI.context(0).check()
+
+
+# ---------------------------------------------------------------------------------------------
+# sizes that reach every layout of lanes, rows per block, run length and a pair's third tile (148 SMs)
+# ---------------------------------------------------------------------------------------------
+def _as_views(c, channels, dev):
+    """u, delta and z as columns of wider rows that start anywhere, B and C as slices of one projection's rows."""
+    import torch
+
+    for key, lead in (("u", 1), ("delta", 3), ("z", channels + 1)):
+        big = torch.zeros(c[key].shape[0], 2 * channels + 5, dtype=c[key].dtype, device=dev)
+        big[:, lead:lead + channels] = c[key]
+        c[key] = big[:, lead:lead + channels]
+    groups, states = c["B"].shape[1:]
+    n = groups * states
+    bc = torch.zeros(c["u"].shape[0], 3 + 2 * n, dtype=c["u"].dtype, device=dev)
+    bc[:, 3:3 + n], bc[:, 3 + n:] = c["B"].flatten(1), c["C"].flatten(1)
+    c["B"], c["C"] = bc[:, 3:3 + n].unflatten(1, (groups, states)), bc[:, 3 + n:].unflatten(1, (groups, states))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("states,channels,groups,views",
+                         [(8, 48, 1, False), (5, 1200, 2, True), (8, 1200, 1, False),       # 8 and 4 lanes for 8 states
+                          (16, 64, 1, False), (13, 800, 1, True), (16, 800, 2, False),      # 16, 8
+                          (16, 1200, 1, False), (16, 1202, 2, True), (13, 1200, 1, False),  # and 4 lanes for 16
+                          (32, 64, 1, True), (24, 800, 1, False), (32, 800, 2, True),       # 16 and 8 lanes for 32
+                          (64, 40, 1, False), (40, 48, 2, True), (128, 40, 1, True), (100, 24, 1, False),
+                          (256, 40, 1, False), (200, 24, 2, True)])
+def test_selective_scan_lanes(KI, dev, dtype, states, channels, groups, views):
+    """Two sequences of four and two chunks of tokens, on every number of lanes per channel and states per lane."""
+    offsets = [0, 37, 140]
+    c, state, slots, initial = _scan_case(states + channels, 143, 2, channels, states, groups, dtype, dev)
+    if views:
+        _as_views(c, channels, dev)
+    initial[:] = False
+    initial[1] = True
+    _scan_check(KI, dev, c, state, slots, initial, offsets)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels,states,groups,views",
+                         [(127, 1024, 8, 1, False), (131, 1030, 5, 2, True), (131, 1200, 16, 1, False), (130, 1030, 13, 2, True),
+                          (67, 1200, 32, 1, False), (66, 1202, 24, 2, True), (35, 600, 64, 1, False), (21, 300, 128, 1, True),
+                          (22, 302, 100, 2, False), (21, 300, 256, 1, False), (23, 301, 200, 1, True)])
+def test_selective_scan_step_four_rows_per_block(KI, dev, dtype, rows, channels, states, groups, views):
+    """Rows enough for four to a block, their number no multiple of four; padding inside a group and at the end."""
+    import torch
+
+    c, state, slots, _ = _scan_case(rows + states, rows, rows, channels, states, groups, dtype, dev)
+    if views:
+        _as_views(c, channels, dev)
+    for r in (1, 6, 8, 9, 10, 11, rows - 1):
+        slots[r] = -1 - r
+    live = [r for r in range(rows) if slots[r] >= 0]
+    want, err, last, lasterr = ref.scan(ref.f64(c["u"]), ref.f64(c["delta"]), ref.f64(c["A"]), ref.f64(c["B"]),
+                                        ref.f64(c["C"]), ref.f64(c["D"]), ref.f64(c["z"]), ref.f64(c["delta_bias"]), True,
+                                        [(r, r + 1) for r in live], [ref.f64(state[int(slots[r])]) for r in live])
+    before = state.clone()
+    out = torch.full(c["u"].shape, 3.0, dtype=c["u"].dtype, device=dev)
+    got = KI.selective_scan_step(**c, state=state, slots=slots.to(dev), out=out)
+    KI.context(0).check()
+    _within(got[live], want[live], err[live], out.dtype)
+    _within(state[slots[live].long().to(dev)], np.stack(last), np.stack(lasterr), torch.float32)
+    named = set(slots[live].tolist())
+    rest = [s for s in range(state.shape[0]) if s not in named]
+    assert torch.equal(state[rest], before[rest])
+    assert (got[[r for r in range(rows) if r not in live]] == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype,channels,width,tokens",
+                         [("bfloat16", 516, 2, 18945), ("bfloat16", 516, 4, 18945), ("bfloat16", 516, 8, 18945),  # runs of 64
+                          ("float32", 258, 3, 18945), ("float16", 129, 4, 18945),
+                          ("bfloat16", 516, 4, 9473), ("float32", 258, 6, 9473), ("float32", 129, 7, 9473),        # of 32
+                          ("float16", 516, 5, 5001)])                                                             # of 16
+def test_causal_conv_long_runs(KI, dev, dtype, channels, width, tokens):
+    """Runs of tokens in which every ring slot is filled many times; sequences that begin a token before, at and after the
+    places where runs begin, short and empty ones among them, continued from their slots."""
+    starts = {64 * i + i % 3 - 1 for i in range(1, 60)} | {16 * i + 1 for i in range(250, 262)} | {32 * i for i in range(140, 150)}
+    offsets = [0, 0] + sorted(starts | {700, 701, 703, 704 + width}) + [tokens - 9, tokens - 9, tokens - 2]
+    x, w, bias, state, slots, initial, off = _conv_case(width, offsets, channels, width, dtype, dev, more=2)
+    slots[5] = -1
+    _conv_check(KI, dev, x, w, bias, state, slots, initial, off, "silu", dtype)
+
+
+@pytest.mark.parametrize("M,N,K", [(3850, 3900, 144), (4609, 4700, 16), (2100, 12800, 48)])
+def test_int8_gemm_of_many_tiles(KI, dev, M, N, K):
+    """Three to seven tiles of 256 x 256 for each CTA pair, so that accumulators and scales are used again, with so few K
+    blocks that the MMAs run ahead of the epilogue; every element."""
+    import torch
+
+    a, w, sa, sw, bias = _operands(M + N + K, M, N, K, dev)
+    s = (a.double() @ w.double().t()) * sa.double()[:, None] * sw.double()  # (the integer sums are exact)
+    for dtype, b in ((torch.float32, None), (torch.bfloat16, bias), (torch.float16, bias)):
+        want = s if b is None else s + b.double()
+        err = 4 * ref.U * s.abs() + (0 if b is None else ref.U * want.abs())
+        bound = err + ref.HALF_STEP[dtype] * (want.abs() + err) + ref.TINY[dtype]
+        big = torch.full((M + 2, N + 3), 5.0, dtype=dtype, device=dev)
+        out = KI.int8_gemm(a, w, sa, sw, bias=b, out=big[1:-1, 1:1 + N])
+        KI.context(0).check()
+        assert torch.isfinite(out).all() and ((out.double() - want).abs() <= bound).all()
+        big[1:-1, 1:1 + N] = 5.0
+        assert (big == 5.0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("channels,width", [(16, 4), (17, 3), (24, 8)])
+def test_causal_conv_of_infinities(KI, dev, dtype, act, channels, width):
+    """Infinities, NaN and values of the type's size in inputs and states stay in the outputs that they reach."""
+    import torch
+
+    T = 30
+    x, w, bias, state, *_ = _conv_case(channels, [0, T], channels, width, dtype, dev, more=0)
+    inf, top = float("inf"), torch.finfo(x.dtype).max
+    w[:, :] = w.abs().clamp(0.1, 0.9)
+    x[5, 0], x[6, 1], x[9, 2] = inf, -inf, float("nan")
+    x[12, 3], x[13, 4] = top, -top
+    x[14, 5], x[15, 5] = inf, -inf
+    state[0, 0, 6], state[0, width - 2, 7] = inf, float("nan")
+    with np.errstate(all="ignore"):
+        want, err, last = ref.conv(ref.f64(x), ref.f64(w), ref.f64(bias), [(0, T)], [ref.f64(state[0])], act == "silu")
+    held, token = state.clone(), state.clone()
+    _as_defined(KI.causal_conv(x, w, bias, state=held, activation=act), want, err, x.dtype)
+    steps = [KI.causal_conv_step(x[t:t + 1], w, bias, state=token, activation=act) for t in range(T)]
+    _as_defined(torch.cat(steps), want, err, x.dtype)
+    assert np.array_equal(ref.f64(held[0]), last[0], equal_nan=True) and torch.equal(held, token)
+    KI.context(0).check()
