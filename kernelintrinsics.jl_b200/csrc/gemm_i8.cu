@@ -49,7 +49,7 @@ template <int BN, bool TMA>
 struct Shape {
     static constexpr int X_BYTES = BN * BK;
     static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
-    // two CTAs per SM, but one with a deeper ring for the widest tiles
+    // two CTAs per SM, but one with a deeper ring for the widest tiles (and where threads load the rows: their registers)
     static constexpr int STAGES = BN <= 16 ? 6 : BN <= 32 ? 5 : BN <= 64 ? 4 : BN <= 128 ? 6 : 5;
     static constexpr int SUM_BYTES = BM * BN * 4;  // a split's Int32 sums, over the ring
     static constexpr int RING_BYTES = STAGES * STAGE_BYTES > SUM_BYTES ? STAGES * STAGE_BYTES : SUM_BYTES;
@@ -660,6 +660,33 @@ int launch_pairs(ki_ctx* ctx, GemmArgs& g, cudaStream_t s) {
     return ki::check_launch(ctx, "gemm_i8_pair_kernel launch");
 }
 
+// Clusters of MAX_SPLIT CTAs that run at once when each CTA takes an SM.
+int clusters_of_eight(ki_ctx* ctx) {
+    if (ctx->gemm_i8_eights == 0) {
+        using S = Shape<128, true>;
+        auto kern = gemm_i8_kernel<128, float, true>;
+        int nc = 0;
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = MAX_SPLIT;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3(MAX_SPLIT * (ctx->sm_count / MAX_SPLIT));
+        cfg.blockDim = dim3(S::THREADS);
+        cfg.dynamicSmemBytes = S::SMEM_BYTES;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM_BYTES) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&nc, kern, &cfg) != cudaSuccess || nc < 1) {
+            cudaGetLastError();
+            nc = ctx->sm_count / 16;
+        }
+        ctx->gemm_i8_eights = nc;
+    }
+    return ctx->gemm_i8_eights;
+}
+
 template <int BN, class O, bool TMA>
 int launch(ki_ctx* ctx, GemmArgs& g, cudaStream_t s) {
     using S = Shape<BN, TMA>;
@@ -673,9 +700,11 @@ int launch(ki_ctx* ctx, GemmArgs& g, cudaStream_t s) {
     const long long tiles = (long long)g.ntiles * g.mtiles;
     if (tiles * MAX_SPLIT > 0x7fffffffll) return ki::set_error(ctx, KI_ERR_ARG, "gemm_i8: too many tiles");
     const int blocks = (g.k + BK - 1) / BK;
-    // Clusters of eight where there are few, or two CTAs fit an SM: sixteen clusters of eight CTAs that need an SM each do not
-    // run at once (128 x 2048 x 4096: 14.9 us in eight parts, 8.8 in four; 1 x 2048 x 4096: 5.8 and 6.3 us).
-    const int most = BN <= 32 || 16 * tiles <= ctx->sm_count ? MAX_SPLIT : 4;
+    // Eight parts where the clusters of eight run at once: two CTAs of up to 32 tokens fit an SM unless threads load the rows; wider
+    // ones take an SM each, and a sixteenth cluster waits for the first fifteen (bf16 out, 15 and 16 tiles of 128 channels:
+    // 128 x 4096 inner 9.6 and 16.7 us in eight parts, 9.8 and 9.9 in four; 1 x 4097 inner 11.1 and 19.7, 15.6 and 15.7).
+    // Tiles of 64 fit twice, but in four parts 16 of them take no longer (48 x 4096 inner 9.3 and 8.8 us; 10 tiles 6.7 and 7.6).
+    const int most = (TMA && BN <= 32) || tiles <= clusters_of_eight(ctx) ? MAX_SPLIT : 4;
     int split = 1;
     while (split < most && 2 * split * tiles <= ctx->sm_count && 2 * split <= blocks) split *= 2;
     auto kern = gemm_i8_kernel<BN, O, TMA>;

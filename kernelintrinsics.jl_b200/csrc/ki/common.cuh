@@ -49,6 +49,7 @@ struct ki_ctx {
     int copy_resident[5] = {};  // resident vcopy blocks per SM, per instantiation
     int gemm_pairs = 0;         // co-resident CTA pairs of the pair GEMM kernel
     int gemm_i8_pairs = 0;      // and of the int8 one
+    int gemm_i8_eights = 0;     // co-resident clusters of eight CTAs of the int8 GEMM, an SM each
     // host-buffer copy pipeline: streams [0] host -> device, [1] kernel, [2] device -> host
     cudaStream_t pipe_stream[3] = {};
     cudaEvent_t pipe_landed[KI_PIPE_SLOTS] = {};   // slot's input chunk is on the device

@@ -1103,3 +1103,16 @@ def test_causal_conv_of_infinities(KI, dev, dtype, act, channels, width):
     _as_defined(torch.cat(steps), want, err, x.dtype)
     assert np.array_equal(ref.f64(held[0]), last[0], equal_nan=True) and torch.equal(held, token)
     KI.context(0).check()
+
+
+@pytest.mark.parametrize("N", [1153, 1920, 1921, 2304])
+@pytest.mark.parametrize("M,K", [(1, 1040), (1, 1031), (48, 1040), (33, 1031), (128, 1040), (100, 1031)])
+def test_int8_gemm_in_clusters(KI, dev, M, N, K):
+    """10 to 18 tiles, whose K blocks are shared by four or eight CTAs."""
+    import torch
+
+    a, w, sa, sw, bias = _operands(M + N + K, M, N, K, dev)
+    for dtype, b in ((torch.float32, None), (torch.bfloat16, bias)):
+        out = KI.int8_gemm(a, w, sa, sw, bias=b, dtype=dtype)
+        KI.context(0).check()
+        _check_product(out, a, w, sa, sw, b, dtype)
