@@ -56,7 +56,8 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& v) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// 2^x with one instruction (2 ulp); results below 2^-126 are zero.
+// 2^x with one instruction (2 ulp); results below 2^-126 are zero, and so are reciprocals of numbers above 2^126: a gate
+// of less than 1.2e-38 (z below -87.3) is zero, as a step or decay of that size is, in Float32 too.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -110,8 +111,9 @@ __device__ __forceinline__ float relu(float x) {
     return y;
 }
 // log(1 + e^x) = max(x, 0) + log1p(e), e = e^-|x| <= 1.  The exponent's product with log2(e) is kept to twice
-// Float32's precision; log1p(e) / e is a polynomial of degree 8, fitted on [0, 1] for the smallest relative error (3e-8;
-// 1.7e-7 with Float32 arithmetic).  No branches, so neighbouring values overlap.
+// Float32's precision; log1p(e) / e is a polynomial of degree 8, fitted on [0, 1] for the smallest relative error (3e-8).
+// With Float32 arithmetic and the fast exponential at most 3.2e-7 off, relative (16 million points of [-87, 100]); zero
+// below -87.3.  No branches, so neighbouring values overlap.
 __device__ __forceinline__ float softplus(float x) {
     const float n = fmaxf(-fabsf(x), -200.0f);
     const float minus = n * -kLog2e;

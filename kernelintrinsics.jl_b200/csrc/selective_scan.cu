@@ -287,7 +287,8 @@ struct Lane {
 };
 
 // The sequence that is rank-th by length, the longest first (equal ones in order): with more blocks than SMs, a long
-// sequence that starts last would run alone at the end.  At most kSort sequences; run by the whole block.
+// sequence that starts last would run alone at the end.  At most kSort sequences, one for each thread; run by the whole
+// block.  (More sequences are taken in order: a longer sort in every block was not tried.)
 constexpr int kSort = kLanes + kHelpers;
 __device__ __forceinline__ int longest(const ki::Sequences& q, int rank, int* lengths) {
     __shared__ int found;
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(kLanes + kHelpers, Tile<T, LPC, K>::NP <= 64 ?
 }
 
 // One token per row: row r continues slot slots[r].  Bound: the states' bytes (one read and one write; 128 x 4096 x 16:
-// 18.2 us, 3.9 TB/s; one row at a time 26.5, two 20.5), so LPC lanes
+// 18.3 us, 3.9 TB/s; one row at a time 26.5, two 20.5), so LPC lanes
 // share a channel with K states each (16 bytes and more per access) and take R rows at once: A is read once for them and
 // their states' loads are in flight together.  What is done once per row and channel (the step, the gate) is done
 // by lane r of the group for row r.
